@@ -101,7 +101,12 @@ enum {
     PAM_OP_PREFILL_TILED_PASS = 4,
     PAM_OP_DECODE = 5,
     PAM_OP_APPEND = 6,
-    PAM_OP_BACKWARD = 7
+    PAM_OP_BACKWARD = 7,
+    PAM_OP_BATCH_PLAN = 8,
+    PAM_OP_QK_NORM_ROPE = 9,
+    PAM_OP_QK_NORM_ROPE_BACKWARD = 10,
+    PAM_OP_TREE_ATTENTION = 11,
+    PAM_OP_TREE_COMMIT = 12
 };
 typedef struct pam_stats {
     int32_t operation;
@@ -447,6 +452,192 @@ typedef struct pam_mixed_request {
     size_t q_bytes, output_bytes, new_keys_bytes, new_values_bytes, k_pool_bytes, v_pool_bytes, block_tables_bytes;
 } pam_mixed_request;
 int32_t pam_engine_mixed_step(void *context, const pam_mixed_request *request);
+
+/* Speculative decoding over the paged cache (no reference counterpart).  A step that
+ * verifies drafted tokens plans the batch on the GPU, norms and rotates the heads on
+ * their way into the cache, attends the drafted trees over it and commits the accepted
+ * path.  Every length, table and mask is a device buffer: a step needs no host value but
+ * the shapes, and its calls can be captured into a HIP graph.
+ *
+ * Capture: after pam_set_synchronous(ctx, false), on a stream set with pam_set_stream,
+ * and with the workspace at its size (the same call once before, or
+ * pam_reserve_workspace); a captured call that would have to allocate is refused.  Graphs
+ * captured from one context share its workspace: replay them one after another, or
+ * capture each from a context of its own.  A later call that needs a larger workspace
+ * leaves the captured one in place until the context is destroyed.
+ *
+ * The calls run on the context's device whatever the current one is.  They are not in
+ * the code object: pam_module_set_strict makes them fail.  Failures are reported, not
+ * degraded from (the outputs are not zero-filled). */
+
+/* Block tables, slot maps, positions and tree masks of a ragged batch from its lengths.
+ * Sequence s holds context_lens[s] cached tokens and gets query_lens[s] new ones; its
+ * ceil((context + new) / block_size) blocks follow those of sequence s - 1 in block_list.
+ * Written whole:
+ *   cu_queries [num_seqs + 1]  rows before each sequence, and their total
+ *   seq_lengths [num_seqs]     context + new (at most the table's tokens)
+ *   block_tables [num_seqs][max_num_blocks], zero padded
+ *   positions [max_rows]       of each new token: context + its depth
+ *   slot_mapping [max_rows]    its pool slot (pam_append_request.slot_mapping)
+ *   tree_mask [max_rows][mask_words], or NULL: bit j of a row: its sequence's new token j is
+ *                              on its path, itself among them
+ * Rows behind the last: position 0, slot -1, mask 0.  parents [parents_len] (NULL: every
+ * sequence's new tokens are a chain) gives each row's parent as an index into its
+ * sequence's new tokens, before its own, or -1 (the cached context); a tree has at most
+ * 1024 nodes, and 64 mask_words when tree_mask is given.  status (optional) gets these
+ * bits or-ed in, so clear it before: 1 more rows than max_rows, 2 blocks past the table's
+ * width or the block list, 4 a negative length (taken as 0), 8 a parent that is no
+ * earlier node (taken as -1) or a tree past its limits.  What does not fit is left out:
+ * nothing is read or written outside the buffers, and the slots of such tokens are -1. */
+typedef struct pam_batch_plan_request {
+    const int32_t *context_lens; /* [num_seqs] */
+    const int32_t *query_lens;   /* [num_seqs] */
+    const int32_t *block_list;   /* [block_list_len] */
+    const int32_t *parents;      /* [parents_len] or NULL */
+    int64_t block_list_len;
+    int64_t parents_len;
+    int32_t num_seqs;
+    int32_t block_size;
+    int32_t max_num_blocks;
+    int32_t max_rows;
+    int32_t mask_words; /* 1 .. 16 with tree_mask */
+    int32_t *cu_queries;
+    uint32_t *seq_lengths;
+    int32_t *block_tables;
+    int32_t *positions;
+    int64_t *slot_mapping;
+    uint64_t *tree_mask;
+    int32_t *status;
+} pam_batch_plan_request;
+int32_t pam_engine_batch_plan(void *context, const pam_batch_plan_request *request);
+
+/* The rotation's pairs: the first rotary_dim dims of a head (even; 0: no rotation) turn by
+ * position * inv_freq[i], pair i being dims (i, i + rotary_dim / 2) or, interleaved,
+ * (2i, 2i + 1).  inv_freq is a host array of rotary_dim / 2 values; NULL: base^(-2i / rotary_dim). */
+typedef struct pam_rotary_spec {
+    int32_t rotary_dim;
+    int32_t interleaved;
+    double base;
+    const double *inv_freq;
+} pam_rotary_spec;
+
+/* RMS norm of every query and key head (y = x / sqrt(mean(x^2) + eps) * weight) with the
+ * rotation to the token's position in the same pass.  Rows are tokens of
+ * layer.num_heads (q) and layer.num_kv_heads (k, values) heads of head_dim, float for f32
+ * layers and half otherwise; strides are elements between rows (0: contiguous), so packed
+ * projections are read in place.  q_out may be q and k_out k, with the same stride.
+ * normalize false: rotation alone.  A NULL weight is ones.  Sums are binary32, angles
+ * exact to 2^-32 of a turn at any position, and an output rounds once.
+ * With k_pool, v_pool and slot_mapping (f32 and f16 layers) the keys and the values'
+ * rows are written to their slots too; tokens of negative slots, or slots past the pools
+ * (k_pool_bytes given), are not; k_out may then be NULL. */
+typedef struct pam_qk_norm_rope_request {
+    const void *q;
+    const void *k;
+    void *q_out;
+    void *k_out;
+    const void *q_weight; /* [head_dim] */
+    const void *k_weight;
+    const int32_t *positions; /* [num_tokens] */
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+    int32_t num_tokens;
+    pam_layer_spec layer;
+    pam_rotary_spec rotary;
+    float eps;
+    bool normalize;
+    const void *values;
+    int64_t v_stride;
+    void *k_pool;
+    void *v_pool;
+    const int64_t *slot_mapping; /* [num_tokens] */
+    size_t q_bytes, k_bytes, q_out_bytes, k_out_bytes, positions_bytes, values_bytes, k_pool_bytes, v_pool_bytes,
+        slot_mapping_bytes;
+} pam_qk_norm_rope_request;
+int32_t pam_engine_qk_norm_rope(void *context, const pam_qk_norm_rope_request *request);
+
+/* Gradients of pam_engine_qk_norm_rope's q_out and k_out: d_q, d_k (written) and the
+ * weights' (float, written; NULL: not wanted), summed over tokens and heads in a fixed
+ * order.  q and k are the forward's inputs. */
+typedef struct pam_qk_norm_rope_backward_request {
+    const void *q;
+    const void *k;
+    const void *d_q_out;
+    const void *d_k_out;
+    void *d_q;
+    void *d_k;
+    const void *q_weight;
+    const void *k_weight;
+    float *d_q_weight; /* [head_dim] */
+    float *d_k_weight;
+    const int32_t *positions;
+    int64_t q_stride, k_stride, d_q_out_stride, d_k_out_stride, d_q_stride, d_k_stride;
+    int32_t num_tokens;
+    pam_layer_spec layer;
+    pam_rotary_spec rotary;
+    float eps;
+    bool normalize;
+    size_t q_bytes, k_bytes, d_q_out_bytes, d_k_out_bytes, d_q_bytes, d_k_bytes, positions_bytes;
+} pam_qk_norm_rope_backward_request;
+int32_t pam_engine_qk_norm_rope_backward(void *context, const pam_qk_norm_rope_backward_request *request);
+
+/* Attention of drafted trees.  Sequence s's rows are cu_queries[s] .. cu_queries[s + 1] - 1
+ * of q and output ([total_rows][num_heads][head_dim]), at most max_queries of them; its
+ * drafted tokens' keys and values are in the pools at positions context_lens[s] + i.  Row i
+ * sees the cached tokens and the drafted tokens whose bits its row of tree_mask
+ * ([total_rows][mask_words]) has set, NULL being a chain (tokens 0 .. i); with a window,
+ * the last window_size of these keys, in order of position.  A row that sees no key is
+ * zeros; rows behind the last sequence are left as they are.  f32, f16 and e4m3 pools. */
+typedef struct pam_tree_attention_request {
+    const void *q;
+    void *output;
+    const void *k_pool;
+    const void *v_pool;
+    const int32_t *block_tables; /* [num_seqs][max_num_blocks] */
+    const int32_t *context_lens; /* [num_seqs] */
+    const int32_t *cu_queries;   /* [num_seqs + 1] */
+    const uint64_t *tree_mask;
+    int32_t mask_words; /* max_queries <= 64 mask_words */
+    int32_t num_seqs;
+    int32_t max_num_blocks;
+    int32_t max_queries;
+    int32_t total_rows;
+    pam_layer_spec layer;
+    const uint16_t *k_scale;
+    const uint16_t *v_scale;
+    /* k_pool_bytes and v_pool_bytes are needed: table entries are held inside the pools */
+    size_t q_bytes, output_bytes, k_pool_bytes, v_pool_bytes, block_tables_bytes, context_lens_bytes,
+        cu_queries_bytes, tree_mask_bytes;
+} pam_tree_attention_request;
+int32_t pam_engine_tree_attention(void *context, const pam_tree_attention_request *request);
+
+/* The accepted path of every sequence moved to the end of its cached tokens: the keys and
+ * values at position context_lens[s] + paths[s][k] go to context_lens[s] + k.  paths is
+ * [num_seqs][max_path]; a path ends at its first entry that is not larger than the one
+ * before or names no new token (a negative one, or query_lens[s] and up).  new_lengths
+ * (optional, not context_lens itself) gets context_lens[s] + the path's length.  e4m3
+ * pools: the path's tokens are appended anew, with the append's scale rule, from the
+ * values that their codes stand for. */
+typedef struct pam_tree_commit_request {
+    void *k_pool;
+    void *v_pool;
+    uint16_t *k_scale;
+    uint16_t *v_scale;
+    const int32_t *block_tables; /* [num_seqs][max_num_blocks] */
+    const int32_t *context_lens; /* [num_seqs] */
+    const int32_t *query_lens;   /* [num_seqs] */
+    const int32_t *paths;
+    int32_t *new_lengths;
+    int32_t num_seqs;
+    int32_t max_num_blocks;
+    int32_t max_path;
+    pam_layer_spec layer;
+    /* k_pool_bytes and v_pool_bytes are needed: nothing is moved outside the pools */
+    size_t k_pool_bytes, v_pool_bytes, block_tables_bytes, context_lens_bytes, query_lens_bytes, paths_bytes;
+} pam_tree_commit_request;
+int32_t pam_engine_tree_commit(void *context, const pam_tree_commit_request *request);
+
+/* The GPU that a context runs on; -1 before its first call that uses one. */
+int32_t pam_context_device(void *context);
 
 /* Code-object loading and launch: the counterpart of the reference's Metal
  * pipeline manager (PagedAttentionEngine.swift:151-198 builds the shader library

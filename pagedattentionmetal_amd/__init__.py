@@ -5,7 +5,7 @@ behind the reference's ``pam_*`` C ABI, declared in ``include/pam.h``).  This
 package mirrors the reference's Swift API over that ABI.
 """
 from .api import (BlockEvictionPolicy, ContinuousBatchingScheduler, KVCacheManager, PagedAttentionDataType,
-                  PagedAttentionEngine, PagedAttentionError, PagedLayerSpec, SequenceStatus)
+                  PagedAttentionEngine, PagedAttentionError, PagedLayerSpec, RotarySpec, SequenceStatus)
 
 __all__ = ["BlockEvictionPolicy", "ContinuousBatchingScheduler", "KVCacheManager", "PagedAttentionDataType",
-           "PagedAttentionEngine", "PagedAttentionError", "PagedLayerSpec", "SequenceStatus"]
+           "PagedAttentionEngine", "PagedAttentionError", "PagedLayerSpec", "RotarySpec", "SequenceStatus"]

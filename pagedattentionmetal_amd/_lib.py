@@ -70,6 +70,53 @@ class MixedRequest(C.Structure):
                 ("block_tables_bytes", SZ)]
 
 
+class BatchPlanRequest(C.Structure):
+    _fields_ = [("context_lens", P), ("query_lens", P), ("block_list", P), ("parents", P), ("block_list_len", I64),
+                ("parents_len", I64), ("num_seqs", I32), ("block_size", I32), ("max_num_blocks", I32),
+                ("max_rows", I32), ("mask_words", I32), ("cu_queries", P), ("seq_lengths", P), ("block_tables", P),
+                ("positions", P), ("slot_mapping", P), ("tree_mask", P), ("status", P)]
+
+
+class RotarySpecC(C.Structure):
+    _fields_ = [("rotary_dim", I32), ("interleaved", I32), ("base", C.c_double), ("inv_freq", P)]
+
+
+class QkNormRopeRequest(C.Structure):
+    _fields_ = [("q", P), ("k", P), ("q_out", P), ("k_out", P), ("q_weight", P), ("k_weight", P), ("positions", P),
+                ("q_stride", I64), ("k_stride", I64), ("q_out_stride", I64), ("k_out_stride", I64),
+                ("num_tokens", I32), ("layer", LayerSpec), ("rotary", RotarySpecC), ("eps", C.c_float),
+                ("normalize", C.c_bool), ("values", P), ("v_stride", I64), ("k_pool", P), ("v_pool", P),
+                ("slot_mapping", P), ("q_bytes", SZ), ("k_bytes", SZ), ("q_out_bytes", SZ), ("k_out_bytes", SZ),
+                ("positions_bytes", SZ), ("values_bytes", SZ), ("k_pool_bytes", SZ), ("v_pool_bytes", SZ),
+                ("slot_mapping_bytes", SZ)]
+
+
+class QkNormRopeBackwardRequest(C.Structure):
+    _fields_ = [("q", P), ("k", P), ("d_q_out", P), ("d_k_out", P), ("d_q", P), ("d_k", P), ("q_weight", P),
+                ("k_weight", P), ("d_q_weight", P), ("d_k_weight", P), ("positions", P), ("q_stride", I64),
+                ("k_stride", I64), ("d_q_out_stride", I64), ("d_k_out_stride", I64), ("d_q_stride", I64),
+                ("d_k_stride", I64), ("num_tokens", I32), ("layer", LayerSpec), ("rotary", RotarySpecC),
+                ("eps", C.c_float), ("normalize", C.c_bool), ("q_bytes", SZ), ("k_bytes", SZ), ("d_q_out_bytes", SZ),
+                ("d_k_out_bytes", SZ), ("d_q_bytes", SZ), ("d_k_bytes", SZ), ("positions_bytes", SZ)]
+
+
+class TreeAttentionRequest(C.Structure):
+    _fields_ = [("q", P), ("output", P), ("k_pool", P), ("v_pool", P), ("block_tables", P), ("context_lens", P),
+                ("cu_queries", P), ("tree_mask", P), ("mask_words", I32), ("num_seqs", I32), ("max_num_blocks", I32),
+                ("max_queries", I32), ("total_rows", I32), ("layer", LayerSpec), ("k_scale", P), ("v_scale", P),
+                ("q_bytes", SZ), ("output_bytes", SZ), ("k_pool_bytes", SZ), ("v_pool_bytes", SZ),
+                ("block_tables_bytes", SZ), ("context_lens_bytes", SZ), ("cu_queries_bytes", SZ),
+                ("tree_mask_bytes", SZ)]
+
+
+class TreeCommitRequest(C.Structure):
+    _fields_ = [("k_pool", P), ("v_pool", P), ("k_scale", P), ("v_scale", P), ("block_tables", P),
+                ("context_lens", P), ("query_lens", P), ("paths", P), ("new_lengths", P), ("num_seqs", I32),
+                ("max_num_blocks", I32), ("max_path", I32), ("layer", LayerSpec), ("k_pool_bytes", SZ),
+                ("v_pool_bytes", SZ), ("block_tables_bytes", SZ), ("context_lens_bytes", SZ),
+                ("query_lens_bytes", SZ), ("paths_bytes", SZ)]
+
+
 class EngineConfig(C.Structure):
     _fields_ = [("split_threshold", I32), ("default_window_size", I32), ("default_chunk_size", I32)]
 
@@ -171,6 +218,12 @@ SIGNATURES = {
     "pam_set_fused_prefill_kernel": (I32, [P, C.c_bool]),
     "pam_set_gpu_timing": (I32, [P, C.c_bool]),
     "pam_engine_mixed_step": (I32, [P, C.POINTER(MixedRequest)]),
+    "pam_engine_batch_plan": (I32, [P, C.POINTER(BatchPlanRequest)]),
+    "pam_engine_qk_norm_rope": (I32, [P, C.POINTER(QkNormRopeRequest)]),
+    "pam_engine_qk_norm_rope_backward": (I32, [P, C.POINTER(QkNormRopeBackwardRequest)]),
+    "pam_engine_tree_attention": (I32, [P, C.POINTER(TreeAttentionRequest)]),
+    "pam_engine_tree_commit": (I32, [P, C.POINTER(TreeCommitRequest)]),
+    "pam_context_device": (I32, [P]),
     "pam_engine_set_config": (I32, [P, C.POINTER(EngineConfig)]),
     "pam_engine_get_config": (I32, [P, C.POINTER(EngineConfig)]),
     "pam_engine_prefill_flat": (I32, [P, C.POINTER(PrefillRequest), I32, I32]),

@@ -782,6 +782,38 @@ PAM_API int32_t pam_engine_mixed_step(void *context, const pam_mixed_request *re
     return guarded(context, [&](Context *ctx) { ctx->mixed_step(*request); });
 }
 
+PAM_API int32_t pam_engine_batch_plan(void *context, const pam_batch_plan_request *request) {
+    if (!request) return -1;
+    return guarded(context, [&](Context *ctx) { ctx->batch_plan(*request); });
+}
+
+PAM_API int32_t pam_engine_qk_norm_rope(void *context, const pam_qk_norm_rope_request *request) {
+    if (!request) return -1;
+    return guarded(context, [&](Context *ctx) { ctx->qk_norm_rope(*request); });
+}
+
+PAM_API int32_t pam_engine_qk_norm_rope_backward(void *context, const pam_qk_norm_rope_backward_request *request) {
+    if (!request) return -1;
+    return guarded(context, [&](Context *ctx) { ctx->qk_norm_rope_backward(*request); });
+}
+
+PAM_API int32_t pam_engine_tree_attention(void *context, const pam_tree_attention_request *request) {
+    if (!request) return -1;
+    return guarded(context, [&](Context *ctx) { ctx->tree_attention(*request); });
+}
+
+PAM_API int32_t pam_engine_tree_commit(void *context, const pam_tree_commit_request *request) {
+    if (!request) return -1;
+    return guarded(context, [&](Context *ctx) { ctx->tree_commit(*request); });
+}
+
+PAM_API int32_t pam_context_device(void *context) {
+    Context *ctx = ctx_of(context);
+    if (!ctx) return -1;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    return ctx->device();
+}
+
 PAM_API int32_t pam_fp8_quantize(void *context, const uint16_t *values, const uint16_t *scales, uint8_t *out,
                                  int64_t n) {
     return guarded(context, [&](Context *ctx) { ctx->fp8_quantize(values, scales, out, n); });

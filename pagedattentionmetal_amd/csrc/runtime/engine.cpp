@@ -13,7 +13,7 @@
 #include <cstdio>
 #include <cstring>
 
-#include "runtime.h"
+#include "engine_util.h"
 
 namespace pam {
 
@@ -26,36 +26,6 @@ void hip_check(hipError_t e, const char *what) {
         throw ExecutionError(std::string("GPU command execution failed: ") + what + ": " + hipGetErrorString(e));
     }
 }
-
-// ------------------------------------------------------------------ helpers
-
-static int32_t elem_bytes(int32_t dtype) { return dtype == kF32 ? 4 : (dtype == kF16 ? 2 : 1); }
-static int32_t io_bytes(int32_t dtype) { return dtype == kF32 ? 4 : 2; }  // Q / O / new K,V element
-
-static void validate_layer(const pam_layer_spec &l) {
-    if (l.head_dim <= 0) throw invalid_configuration("headDim must be positive.");
-    if (l.num_heads <= 0) throw invalid_configuration("numHeads must be positive.");
-    if (l.num_kv_heads <= 0) throw invalid_configuration("numKVHeads must be positive.");
-    if (l.num_heads % l.num_kv_heads != 0)
-        throw invalid_configuration("numHeads must be divisible by numKVHeads for GQA/MQA mapping.");
-    if (l.block_size <= 0) throw invalid_configuration("blockSize must be positive.");
-    if (l.data_type < 0 || l.data_type > 2) throw invalid_configuration("unknown dtype");
-    if (l.window_size < 0) throw invalid_configuration("windowSize must be non-negative.");
-    // kernel envelope: 4-element slices per lane, at most 64 lanes per token row
-    if (l.head_dim % 4 != 0 || l.head_dim > 256)
-        throw PamError("Unsupported paged attention path: headDim must be a multiple of 4 and at most 256.");
-}
-
-static void require(size_t actual, const char *name, int64_t expected) {
-    if (actual != 0 && (int64_t)actual < expected) throw buffer_too_small(name, expected, (int64_t)actual);
-}
-
-static int64_t q_bytes_per_token(const pam_layer_spec &l) { return (int64_t)l.num_heads * l.head_dim * io_bytes(l.data_type); }
-static int64_t kv_bytes_per_token(const pam_layer_spec &l) {
-    return (int64_t)l.num_kv_heads * l.head_dim * elem_bytes(l.data_type);
-}
-static int64_t pool_bytes_for(int64_t blocks, const pam_layer_spec &l) { return blocks * l.block_size * kv_bytes_per_token(l); }
-static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The prefill regime lastStats.operation names, by the reference's rule
 // (PagedAttentionEngine.swift:420-433, 436-438, 512-516, 1952-1958): MMA for f16
@@ -83,6 +53,7 @@ Context::~Context() {
     module_unload();
     if (own_stream_) (void)hipStreamSynchronize(own_stream_);
     if (workspace_.ptr) (void)hipFree(workspace_.ptr);
+    for (void *w : workspace_kept_) (void)hipFree(w);
     if (seg_count_.ptr) (void)hipFree(seg_count_.ptr);
     for (auto &s : scratch_)
         if (s.ptr) (void)hipFree(s.ptr);
@@ -148,7 +119,11 @@ void Context::reserve_workspace(size_t bytes) {
     if (bytes <= workspace_.bytes) return;
     hip_check(hipStreamSynchronize(stream()), "workspace resize");
     const size_t want = grown(bytes, workspace_.bytes);
-    if (workspace_.ptr) (void)hip_check(hipFree(workspace_.ptr), "hipFree");
+    if (workspace_.ptr && workspace_captured_)
+        workspace_kept_.push_back(workspace_.ptr);
+    else if (workspace_.ptr)
+        hip_check(hipFree(workspace_.ptr), "hipFree");
+    workspace_captured_ = false;
     workspace_.ptr = nullptr;
     workspace_.bytes = 0;
     hip_check(hipMalloc(&workspace_.ptr, want), "hipMalloc workspace");
@@ -257,6 +232,20 @@ void Context::check_launch(F &&launch, const char *what) {
     }
     const hipError_t e = launch();
     if (e != hipSuccess) throw PamError(std::string("GPU command encoding failed: ") + what + ": " + hipGetErrorString(e));
+}
+
+// One call's launches as a retried unit with its timing and stats (speculative.cpp).
+void Context::run_spec(const char *op, int32_t stats_op, int32_t batch, int32_t rows, int64_t tmp, bool capturing,
+                       const std::function<hipError_t()> &launch) {
+    const bool timed = gpu_timing && !capturing;
+    with_retry(op, [&] {
+        if (timed) mark(ev0_);
+        check_launch(launch, op);
+        if (timed) mark(ev1_);
+        finish(op);
+    });
+    record_stats(stats_op, batch, rows, 0, tmp, false, false);
+    if (!timed) stats_pending_ = false;
 }
 
 void Context::zero_output(void *ptr, size_t bytes) {

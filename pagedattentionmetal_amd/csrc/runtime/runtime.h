@@ -11,13 +11,14 @@
 
 #include <cstdint>
 #include <cstring>
+#include <functional>
 #include <mutex>
 #include <string>
 #include <unordered_map>
 #include <vector>
 
 #include "../../../include/pam.h"
-#include "../kernels/kernels.h"
+#include "../kernels/speculative.h"
 #include "block_allocator.h"
 
 namespace pam {
@@ -134,6 +135,13 @@ class Context {
     void mixed_step(const pam_mixed_request &r);
     void fused_prefill(const pam_fused_prefill_request &r);
     void backward(const pam_backward_request &r);
+    // --- speculative decoding (speculative.cpp)
+    void batch_plan(const pam_batch_plan_request &r);
+    void qk_norm_rope(const pam_qk_norm_rope_request &r);
+    void qk_norm_rope_backward(const pam_qk_norm_rope_backward_request &r);
+    void tree_attention(const pam_tree_attention_request &r);
+    void tree_commit(const pam_tree_commit_request &r);
+    int device() const { return device_ready_ ? device_ : -1; }
     void fp8_quantize(const uint16_t *v, const uint16_t *s, uint8_t *o, int64_t n);
     void fp8_dequant(const uint8_t *c, const uint16_t *s, uint16_t *o, int64_t n);
 
@@ -200,6 +208,10 @@ class Context {
     void with_retry(const char *op, F &&fn);
     template <class F>
     void check_launch(F &&launch, const char *what);
+    void run_spec(const char *op, int32_t stats_op, int32_t batch, int32_t rows, int64_t tmp, bool capturing,
+                  const std::function<hipError_t()> &launch);
+    bool begin_spec();
+    void spec_workspace(size_t bytes, bool capturing);
     void zero_output(void *ptr, size_t bytes);
     void decode_checked(const pam_decode_request &r, bool noalloc);
     void decode_gpu(const pam_decode_request &r, char *fixed);
@@ -261,6 +273,10 @@ class Context {
     bool stats_pending_ = false;
     bool stats_has_mid_ = false;
     DeviceBuffer workspace_;
+    // a captured graph holds the workspace's address: a larger one is then allocated
+    // beside it, and it is freed with the context
+    bool workspace_captured_ = false;
+    std::vector<void *> workspace_kept_;
     DeviceBuffer seg_count_;  // stream-K merge counters (epoch-tagged, never reset)
     DeviceBuffer pf_part_;    // dense prefill: partial slots of split items
     DeviceBuffer pf_count_;   // dense prefill: merge counters (epoch-tagged, never reset)
