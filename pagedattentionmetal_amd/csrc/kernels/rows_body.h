@@ -255,16 +255,30 @@ struct RowTiles {
     }
 
     // Tiles t0, t0 + step, .. below t1.  k_hi[b]: end of the keys of row n of block b.
+    struct Ends {
+        const int (&k_hi)[RB];
+        __device__ __forceinline__ bool sees(int b, int j) const { return j < k_hi[b]; }
+        __device__ __forceinline__ int32_t block(int32_t entry) const { return entry; }
+        __device__ __forceinline__ int lo_all(const TileKeys &keys) const { return keys.lo; }
+    };
     __device__ __forceinline__ void run(const AttnParams &p, const TileKeys &keys, const int (&k_hi)[RB], int t0, int t1,
                                         int step) {
+        run(p, keys, Ends{k_hi}, t0, t1, step);
+    }
+    // The same with the keys of row n of block b by see.sees(b, key), asked in tiles that
+    // some row does not see whole (keys from see.lo_all to keys.hi_all are seen by every
+    // row), and table entries by see.block(entry).
+    template <typename See>
+    __device__ __forceinline__ void run(const AttnParams &p, const TileKeys &keys, const See &see, int t0, int t1,
+                                        int step) {
         if (t0 >= t1) return;
-        const int bs = keys.block_size;
+        const int bs = keys.block_size, lo_all = see.lo_all(keys);
         auto lookup = [&](int t, int &slot) {
             int j = keys.key0 + 16 * t + n;
             j = j < keys.lo ? keys.lo : (j < keys.hi ? j : keys.hi - 1);
             const int b = keys.shift >= 0 ? j >> keys.shift : j / bs;
             slot = j - b * bs;
-            return keys.bt[b];
+            return see.block(keys.bt[b]);
         };
         int slot, block = lookup(t0, slot), slot_n = 0, block_n = 0;
         if (t0 + step < t1) block_n = lookup(t0 + step, slot_n);
@@ -304,7 +318,7 @@ struct RowTiles {
             // passes it by 8, a factor of 2^8 (or the row has none yet): the probabilities
             // are f32, so their scale is free, and most tiles need no reduction across
             // lanes.
-            const bool full = kb >= keys.lo && kb + 16 <= keys.hi_all;
+            const bool full = kb >= lo_all && kb + 16 <= keys.hi_all;
             bool grow = false;
 #pragma unroll
             for (int b = 0; b < RB; b++) {
@@ -313,7 +327,7 @@ struct RowTiles {
                     float x = s[b][r] * p.scale_log2;
                     if (!full) {
                         const int j = kb + 4 * g + r;
-                        x = j >= keys.lo && j < keys.hi && j < k_hi[b] ? x : -INFINITY;
+                        x = j >= keys.lo && j < keys.hi && see.sees(b, j) ? x : -INFINITY;
                     }
                     s[b][r] = x;
                     grow |= x > m[b] + 8.0f;
@@ -347,7 +361,7 @@ struct RowTiles {
             // it); add_odd gives the others to the rows that do see the key.
             auto hide = [&](int r, float &x) {
                 const int j = kb + 4 * g + r;
-                const bool bad = !(j >= keys.lo && j < keys.hi_all) && !__builtin_isfinite(x);
+                const bool bad = !(j >= lo_all && j < keys.hi_all) && !__builtin_isfinite(x);
                 odd |= bad;
                 x = bad ? 0.0f : x;
             };

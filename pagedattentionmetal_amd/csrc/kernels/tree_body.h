@@ -114,4 +114,213 @@ __device__ __forceinline__ int tree_first_key(const TreeParams &p, const TreeSeq
     return p.a.window > 0 && first > 0 ? (int)first : 0;
 }
 
+// ------------------------------------------------------------------ the split
+// The work is cut into units: block_rows query rows (token, head) of one kv head and
+// unit_keys keys.  An item is a row block with all its keys; items lie one behind the other
+// (sequence, kv head, block), and every workgroup takes the same number of units, wherever
+// items begin and end.  Lengths are known on the device alone, so each workgroup adds
+// them up itself (a wave at a time, 64 sequences a step).  An item that several workgroups
+// share leaves a partial each, which tree_reduce_kernel merges in order: no counters, no
+// atomics, the same bits every time.
+struct TreeWork {
+    int64_t units, per;  // all units, and units of a workgroup
+};
+struct TreeItem {
+    TreeSeq q;
+    int s, kvh, rb;          // sequence, kv head, row block
+    int blocks, waves;       // row blocks of a kv head; 16- or 32-row parts of a block in use
+    int tile0, tiles;        // first key's unit and units of the item
+    int64_t first;           // its first unit
+};
+
+__device__ __forceinline__ int tree_row_blocks(const TreeParams &p, int n) {
+    const int64_t rows = (int64_t)n * (p.a.num_heads / p.a.num_kv_heads);
+    return (int)((rows + p.block_rows - 1) / p.block_rows);
+}
+__device__ __forceinline__ void tree_tiles(const TreeParams &p, const TreeSeq &q, int &tile0, int &tiles) {
+    tile0 = tree_first_key(p, q) / p.unit_keys;
+    tiles = (q.hi + p.unit_keys - 1) / p.unit_keys - tile0;
+    if (tiles < 1) tiles = 1;  // a row without keys is written too
+}
+__device__ __forceinline__ int64_t tree_units(const TreeParams &p, int s) {
+    if (s >= p.num_seqs) return 0;
+    const TreeSeq q = tree_seq(p, s);
+    int tile0, tiles;
+    tree_tiles(p, q, tile0, tiles);
+    return (int64_t)tree_row_blocks(p, q.n) * p.a.num_kv_heads * tiles;
+}
+__device__ __forceinline__ TreeWork tree_work(const TreeParams &p) {
+    int64_t t = 0;
+    for (int s = threadIdx.x & 63; s < p.num_seqs; s += 64) t += tree_units(p, s);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
+    TreeWork w;
+    w.units = t;
+    w.per = (t + p.groups - 1) / p.groups;
+    if (w.per < p.min_units) w.per = p.min_units;
+    return w;
+}
+__device__ __forceinline__ void tree_enter(const TreeParams &p, int s, TreeItem &it) {
+    it.s = s;
+    it.q = tree_seq(p, s);
+    it.blocks = tree_row_blocks(p, it.q.n);
+    tree_tiles(p, it.q, it.tile0, it.tiles);
+}
+// the item that holds unit u (u < units)
+__device__ __forceinline__ void tree_find(const TreeParams &p, int64_t u, TreeItem &it) {
+    const int lane = threadIdx.x & 63;
+    int64_t base = 0;
+    int s = 0;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+        const int64_t mine = tree_units(p, s0 + lane);
+        int64_t upto = mine;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int64_t o = __shfl_up(upto, m, 64);
+            if (lane >= m) upto += o;
+        }
+        const uint64_t past = __ballot(base + upto > u);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            s = s0 + at;
+            base += __shfl(upto - mine, at, 64);
+            break;
+        }
+        base += __shfl(upto, 63, 64);
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    tree_enter(p, s, it);
+    const int64_t k = (u - base) / it.tiles;  // item of the sequence
+    it.kvh = (int)(k / it.blocks);
+    it.rb = (int)(k % it.blocks);
+    it.first = base + k * it.tiles;
+}
+// the item behind it, when there is one
+__device__ __forceinline__ void tree_next(const TreeParams &p, TreeItem &it) {
+    it.first += it.tiles;
+    if (++it.rb < it.blocks) return;
+    it.rb = 0;
+    if (++it.kvh < p.a.num_kv_heads) return;
+    it.kvh = 0;
+    do {
+        if (it.s + 1 >= p.num_seqs) return;
+        tree_enter(p, it.s + 1, it);
+    } while (it.blocks == 0);
+}
+// rows of a block: the item's parts of `part` rows are dealt evenly over its blocks
+struct TreeRows {
+    int row0, rows;  // of the sequence's n G rows of the kv head
+};
+__device__ __forceinline__ TreeRows tree_rows(const TreeParams &p, const TreeItem &it, int part) {
+    const int n = it.q.n * (p.a.num_heads / p.a.num_kv_heads);
+    const int parts = (n + part - 1) / part, per = (parts + it.blocks - 1) / it.blocks * part;
+    TreeRows r;
+    r.row0 = it.rb * per;
+    r.rows = n - r.row0 < per ? n - r.row0 : per;
+    if (r.rows < 0) r.rows = 0;
+    return r;
+}
+// the slot of workgroup w's partial of an item that begins at unit `first`
+__device__ __forceinline__ int64_t tree_slot(const TreeWork &w, int64_t group, int64_t first) {
+    return 2 * group + (first <= group * w.per ? 0 : 1);
+}
+__device__ __forceinline__ float *tree_part_o(const TreeParams &p, int64_t slot) {
+    return p.a.part_o + slot * p.block_rows * (p.a.head_dim + 2);
+}
+__device__ __forceinline__ float *tree_part_ml(const TreeParams &p, int64_t slot) {
+    return tree_part_o(p, slot) + (int64_t)p.block_rows * p.a.head_dim;
+}
+
+// 4 dims of a row from N states of it: O at o + i o_stride (unscaled, reference max m),
+// (m, l) at ml + i ml_stride
+struct TreeSum {
+    float a[4], den, M;
+};
+__device__ __forceinline__ TreeSum tree_sum(const float *o, int64_t o_stride, const float *ml, int64_t ml_stride, int n) {
+    TreeSum s{{0.f, 0.f, 0.f, 0.f}, 0.0f, -INFINITY};
+    for (int i = 0; i < n; i++) s.M = fmaxf(s.M, ml[i * ml_stride]);
+    const float mu = s.M == -INFINITY ? 0.0f : s.M;
+    for (int i = 0; i < n; i++) {
+        const float w = exp2f(ml[i * ml_stride] - mu);  // 0 for a state without keys
+        const float4 v = *reinterpret_cast<const float4 *>(o + i * o_stride);
+        s.den += w * ml[i * ml_stride + 1];
+        s.a[0] += w * v.x, s.a[1] += w * v.y, s.a[2] += w * v.z, s.a[3] += w * v.w;
+    }
+    return s;
+}
+template <typename QT>
+__device__ __forceinline__ void tree_out(const TreeParams &p, const TreeItem &it, int row, int e0, TreeSum &s) {
+    const int H = p.a.num_heads, G = H / p.a.num_kv_heads;
+    const float inv = s.den == 0.0f ? 0.0f : 1.0f / s.den;
+#pragma unroll
+    for (int e = 0; e < 4; e++) s.a[e] *= inv;
+    const int64_t at = ((int64_t)(it.q.row0 + row / G) * H + it.kvh * G + row % G) * p.a.head_dim + e0;
+    store4<QT>(static_cast<QT *>(p.a.out) + at, s.a);
+}
+
+// The V elements left out of the products: not finite, of keys [j0, j1) outside [lo_all,
+// c), which some rows do not see.  Adds p v to 4 dims of a row that sees them.
+template <typename KV, typename QT>
+__device__ __forceinline__ void tree_odd(const TreeParams &p, const TreeItem &it, int row, int e0, int j0, int j1,
+                                         int lo_all, TreeSum &s) {
+    const AttnParams &a = p.a;
+    const int G = a.num_heads / a.num_kv_heads, d = a.head_dim, bs = a.block_size;
+    TreeRow r;
+    r.init(p, it.q, row / G);
+    const QT *qr = static_cast<const QT *>(a.q) +
+                   ((int64_t)(it.q.row0 + row / G) * a.num_heads + it.kvh * G + row % G) * d;
+    const float mu = s.M == -INFINITY ? 0.0f : s.M;
+    for (int j = j0; j < j1; j++) {
+        if (j >= lo_all && j < it.q.c) {
+            j = it.q.c - 1;
+            continue;
+        }
+        if (!r.sees(j, it.q.c)) continue;
+        const int blk = tree_block(p, it.q.bt[j / bs]);
+        const int64_t off = (pool_slot(blk, bs, j % bs) * a.num_kv_heads + it.kvh) * d;
+        f16 ks = (f16)1.0f, vs = (f16)1.0f;
+        if constexpr (sizeof(KV) == 1) ks = bits_to_f16(a.k_scale[blk]), vs = bits_to_f16(a.v_scale[blk]);
+        float v[4];
+        load_kv4<KV>(static_cast<const KV *>(a.v_pool) + off + e0, vs, v);
+        if (__builtin_isfinite(v[0]) && __builtin_isfinite(v[1]) && __builtin_isfinite(v[2]) && __builtin_isfinite(v[3]))
+            continue;
+        float sd = 0.0f;
+        for (int e = 0; e < d; e += 4) {
+            float kv[4], qv[4];
+            load_kv4<KV>(static_cast<const KV *>(a.k_pool) + off + e, ks, kv);
+            load4<QT>(qr + e, qv);
+            sd += qv[0] * kv[0] + qv[1] * kv[1] + qv[2] * kv[2] + qv[3] * kv[3];
+        }
+        const float pj = exp2f(sd * a.scale_log2 - mu);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (!__builtin_isfinite(v[e])) s.a[e] += pj * v[e];
+    }
+}
+
+// A workgroup's rows in LDS (`n` states a row) as outputs, or as the workgroup's partial
+// of an item that others share.
+template <typename KV, typename QT, int ROWS_STRIDE>
+__device__ __forceinline__ void tree_write(const TreeParams &p, const TreeItem &it, const TreeRows &tr, const TreeWork &w,
+                                           int64_t group, int64_t u0, int64_t u1, const float *o, int64_t o_stride,
+                                           const float *ml, int64_t ml_stride, int states, bool any_odd, int lo_all) {
+    const int d = p.a.head_dim, pieces = d / 4;
+    const bool whole = u0 == it.first && u1 == it.first + it.tiles;
+    const int64_t slot = tree_slot(w, group, u0);
+    float *po = tree_part_o(p, slot), *pml = tree_part_ml(p, slot);
+    const int j0 = (it.tile0 + (int)(u0 - it.first)) * p.unit_keys;
+    const int j1e = (it.tile0 + (int)(u1 - it.first)) * p.unit_keys, j1 = j1e < it.q.hi ? j1e : it.q.hi;
+    for (int i = threadIdx.x; i < tr.rows * pieces; i += blockDim.x) {
+        const int r = i / pieces, e0 = (i - r * pieces) * 4;
+        TreeSum s = tree_sum(o + r * ROWS_STRIDE + e0, o_stride, ml + r * 2, ml_stride, states);
+        if (any_odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1, lo_all, s);
+        if (whole) {
+            tree_out<QT>(p, it, tr.row0 + r, e0, s);
+        } else {
+            store4<float>(po + (int64_t)r * d + e0, s.a);
+            if (e0 == 0) *reinterpret_cast<float2 *>(pml + 2 * r) = make_float2(s.M, s.den);
+        }
+    }
+}
+
 }  // namespace pam

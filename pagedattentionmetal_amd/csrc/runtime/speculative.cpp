@@ -312,7 +312,10 @@ void Context::tree_attention(const pam_tree_attention_request &r) {
     p.num_seqs = r.num_seqs;
     p.max_queries = r.max_queries;
     p.total_rows = r.total_rows;
-    run_spec("treeAttention", PAM_OP_TREE_ATTENTION, r.num_seqs, r.total_rows, 0, capturing,
+    const int64_t tmp = tree_plan(p, l.data_type, cus_);
+    spec_workspace((size_t)tmp, capturing);
+    a.part_o = static_cast<float *>(workspace_.ptr);
+    run_spec("treeAttention", PAM_OP_TREE_ATTENTION, r.num_seqs, r.total_rows, tmp, capturing,
              [&] { return launch_tree_attention(p, l.data_type, stream()); });
 }
 
