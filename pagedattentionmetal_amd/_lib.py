@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpam.so")
@@ -115,6 +116,25 @@ class TreeCommitRequest(C.Structure):
                 ("max_num_blocks", I32), ("max_path", I32), ("layer", LayerSpec), ("k_pool_bytes", SZ),
                 ("v_pool_bytes", SZ), ("block_tables_bytes", SZ), ("context_lens_bytes", SZ),
                 ("query_lens_bytes", SZ), ("paths_bytes", SZ)]
+
+
+def packer(cls):
+    """struct.Struct.pack of a request's fields in order, nested ones in place (0 for a null pointer): the bytes of the
+    C struct, for a fraction of what filling the ctypes structure costs."""
+    codes = {P: "Q", I32: "i", I64: "q", SZ: "Q", C.c_float: "f", C.c_double: "d", C.c_bool: "?"}
+    fmt, at = "=", 0
+
+    def walk(c, base):
+        nonlocal fmt, at
+        for name, t in c._fields_:
+            off = base + getattr(c, name).offset
+            if issubclass(t, C.Structure):
+                walk(t, off)
+            else:
+                fmt += "x" * (off - at) + codes[t]
+                at = off + C.sizeof(t)
+    walk(cls, 0)
+    return struct.Struct(fmt + "x" * (C.sizeof(cls) - at)).pack
 
 
 class EngineConfig(C.Structure):
@@ -279,3 +299,10 @@ def load() -> C.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def raw(name: str):
+    """A request call as a function object of its own that takes the packed request's bytes."""
+    fn = load()[name]
+    fn.restype, fn.argtypes = I32, [P, P]
+    return fn

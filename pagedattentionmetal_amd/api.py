@@ -10,11 +10,12 @@ libpam's HIP kernels.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 from enum import IntEnum
 
 from . import _lib
+from .errors import PagedAttentionError
+from .speculative import RotarySpec, SpeculativeCalls  # noqa: F401  (RotarySpec: part of this module's surface)
 
 L = None
 
@@ -39,10 +40,6 @@ class PagedAttentionDataType(IntEnum):
     @property
     def is_quantized(self) -> bool:
         return self == PagedAttentionDataType.float8
-
-
-class PagedAttentionError(RuntimeError):
-    """PagedAttentionError / KVCacheError text from pam_last_error."""
 
 
 class BlockEvictionPolicy(IntEnum):
@@ -88,33 +85,6 @@ class PagedLayerSpec:
                               self.window_size)
 
 
-class RotarySpec:
-    """The position rotation of query and key heads: the first ``rotary_dim`` dims of a head (even) turn by
-    position * inv_freq[i], pair i being dims (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).
-    ``inv_freq`` (rotary_dim / 2 numbers) replaces base^(-2i / rotary_dim)."""
-
-    def __init__(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, inv_freq=None):
-        rotary_dim = int(rotary_dim)
-        if rotary_dim < 0 or rotary_dim % 2:
-            raise PagedAttentionError("Invalid paged attention configuration: rotaryDim must be even and at most "
-                                      "headDim.")
-        if inv_freq is None:
-            if not (math.isfinite(base) and base > 0):
-                raise PagedAttentionError("Invalid paged attention configuration: the rotation's base must be "
-                                          "positive.")
-            inv_freq = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-        freq = [float(f) for f in inv_freq]
-        if len(freq) != rotary_dim // 2 or not all(math.isfinite(f) for f in freq):
-            raise PagedAttentionError("Invalid paged attention configuration: inv_freq needs rotary_dim / 2 finite "
-                                      "numbers.")
-        self.rotary_dim, self.base, self.interleaved, self.inv_freq = rotary_dim, float(base), bool(interleaved), freq
-        self._freq = (C.c_double * max(1, len(freq)))(*freq)
-        self._c = _lib.RotarySpecC(rotary_dim, int(self.interleaved), self.base, C.addressof(self._freq))
-
-    def c(self) -> _lib.RotarySpecC:
-        return self._c
-
-
 def _ptr(t):
     if t is None:
         return None
@@ -139,7 +109,7 @@ class _DeviceArray:
                                          "version": 2, "strides": None}
 
 
-class PagedAttentionEngine:
+class PagedAttentionEngine(SpeculativeCalls):
     """PagedAttentionEngine (PagedAttentionEngine.swift).  One libpam context: one
     HIP stream, synchronous calls unless ``synchronous = False``."""
 
@@ -456,181 +426,6 @@ class PagedAttentionEngine:
             cl.ctypes.data_as(C.c_void_p), ql.ctypes.data_as(C.c_void_p), layer.c(), _nbytes(q), _nbytes(output),
             _nbytes(new_keys), _nbytes(new_values), _nbytes(k_pool), _nbytes(v_pool), _nbytes(block_tables))
         self._check(lib().pam_engine_mixed_step(self._ctx, C.byref(r)))
-
-    # --- speculative decoding (no reference counterpart)
-    def _device_args(self, dtypes, **tensors):
-        """Checks of device buffers: on one GPU (the engine's, once it has one), contiguous, of their type."""
-        dev = None
-        for name, t in tensors.items():
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise PagedAttentionError(f"Invalid paged attention configuration: {name} is not on a GPU.")
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                raise PagedAttentionError(f"Invalid paged attention configuration: {name} is on another GPU.")
-            if t.dtype not in dtypes:
-                raise PagedAttentionError(f"Invalid paged attention configuration: {name} is {t.dtype}.")
-            if not t.is_contiguous():
-                raise PagedAttentionError("buffers must be contiguous")
-        if dev is not None:
-            have = lib().pam_context_device(self._ctx)
-            if have < 0:  # the context takes the buffers' GPU
-                import torch
-                if torch.cuda.current_device() != dev.index:
-                    raise PagedAttentionError("Invalid paged attention configuration: the engine's first call needs "
-                                              "its buffers' GPU as the current one.")
-            elif have != dev.index:
-                raise PagedAttentionError("Invalid paged attention configuration: the buffers are on another GPU "
-                                          "than the engine.")
-
-    @staticmethod
-    def _want(ok, message):
-        if not ok:
-            raise PagedAttentionError("Invalid paged attention configuration: " + message)
-
-    def batch_plan(self, context_lens, query_lens, block_list, block_size, cu_queries, seq_lengths, block_tables,
-                   positions, slot_mapping, parents=None, tree_mask=None, status=None):
-        """Block tables, slot maps, positions and tree masks of a ragged batch, built on the GPU from its lengths
-        (pam_engine_batch_plan).  int32 device tensors, slot_mapping and tree_mask int64; all but status are
-        written whole: block_tables [sequences, width], positions and slot_mapping [rows at most], tree_mask
-        [rows at most, words].  ``parents``: each row's parent among its sequence's new tokens, -1 for none."""
-        import torch
-        i32, i64 = (torch.int32,), (torch.int64,)
-        self._device_args(i32, context_lens=context_lens, query_lens=query_lens, block_list=block_list,
-                          cu_queries=cu_queries, seq_lengths=seq_lengths, block_tables=block_tables,
-                          positions=positions, parents=parents, status=status)
-        self._device_args(i64, slot_mapping=slot_mapping, tree_mask=tree_mask)
-        n, rows = context_lens.numel(), positions.numel()
-        self._want(query_lens.numel() == n and cu_queries.numel() == n + 1 and seq_lengths.numel() == n,
-                   f"the lengths of {n} sequences do not match.")
-        self._want(block_tables.dim() == 2 and block_tables.shape[0] == n, "block_tables needs one row per sequence.")
-        self._want(slot_mapping.numel() == rows, "positions and slot_mapping need the same rows.")
-        self._want(tree_mask is None or (tree_mask.dim() == 2 and tree_mask.shape[0] == rows),
-                   "tree_mask needs one row per position.")
-        r = _lib.BatchPlanRequest(
-            _ptr(context_lens), _ptr(query_lens), _ptr(block_list), _ptr(parents), block_list.numel(),
-            0 if parents is None else parents.numel(), n, int(block_size), block_tables.shape[1], rows,
-            0 if tree_mask is None else tree_mask.shape[1], _ptr(cu_queries), _ptr(seq_lengths), _ptr(block_tables),
-            _ptr(positions), _ptr(slot_mapping), _ptr(tree_mask), _ptr(status))
-        self._check(lib().pam_engine_batch_plan(self._ctx, C.byref(r)))
-
-    def _rows(self, name, t, heads, layer, tokens, io):
-        """A [tokens, heads, head_dim] tensor whose heads are contiguous: its pointer and row stride."""
-        self._want(t.is_cuda, f"{name} is not on a GPU.")
-        self._want(t.dtype == io, f"{name} is {t.dtype}, expected {io}.")
-        d = layer.head_dim
-        self._want(tuple(t.shape) == (tokens, heads, d), f"{name} is {list(t.shape)}, expected "
-                   f"{[tokens, heads, d]}.")
-        s = t.stride()
-        self._want(s[2] == 1 and (s[1] == d or heads == 1) and (tokens == 1 or s[0] >= heads * d),
-                   f"{name}'s heads must be contiguous.")
-        return t.data_ptr(), (s[0] if tokens > 1 else heads * d)
-
-    def _norm_args(self, layer, q, positions, q_weight, k_weight, normalize, rotary):
-        import torch
-        io = torch.float32 if layer.data_type == PagedAttentionDataType.float32 else torch.float16
-        n = q.shape[0]
-        self._device_args((torch.int32,), positions=positions)
-        self._device_args((io,), q_weight=q_weight, k_weight=k_weight)
-        self._want(positions is None or positions.numel() == n, "positions need one entry per token.")
-        for w in (q_weight, k_weight):
-            self._want(w is None or w.numel() == layer.head_dim, "weights have head_dim entries.")
-        return io, n, rotary.c() if rotary is not None else _lib.RotarySpecC(0, 0, 1.0, None)
-
-    def qk_norm_rope(self, q, k, q_out, k_out, positions, layer: PagedLayerSpec, q_weight=None, k_weight=None,
-                     eps: float = 1e-6, rotary: RotarySpec = None, normalize: bool = True, values=None, k_pool=None,
-                     v_pool=None, slot_mapping=None):
-        """RMS norm of every query and key head and the rotation to its token's position in one pass
-        (pam_engine_qk_norm_rope).  q, k, values and the outputs are [tokens, heads, head_dim] of any row stride;
-        q_out may be q, k_out k.  With the pools and an int64 slot_mapping the keys and values go to their slots
-        too, and k_out may be None."""
-        import torch
-        io, n, rot = self._norm_args(layer, q, positions, q_weight, k_weight, normalize, rotary)
-        K = layer.num_kv_heads
-        qp, qs = self._rows("q", q, layer.num_heads, layer, n, io)
-        kp, ks = self._rows("k", k, K, layer, n, io)
-        qo, qos = self._rows("q_out", q_out, layer.num_heads, layer, n, io)
-        ko, kos = self._rows("k_out", k_out, K, layer, n, io) if k_out is not None else (None, 0)
-        vp, vs = self._rows("values", values, K, layer, n, io) if values is not None else (None, 0)
-        self._device_args((io,), q_out=q_out if q_out.is_contiguous() else None, k_pool=k_pool, v_pool=v_pool)
-        self._device_args((torch.int64,), slot_mapping=slot_mapping)
-        self._want(slot_mapping is None or slot_mapping.numel() == n, "slot_mapping needs one entry per token.")
-        r = _lib.QkNormRopeRequest(
-            qp, kp, qo, ko, _ptr(q_weight), _ptr(k_weight), _ptr(positions), qs, ks, qos, kos, n, layer.c(), rot,
-            float(eps), bool(normalize), vp, vs, _ptr(k_pool), _ptr(v_pool), _ptr(slot_mapping), 0, 0, 0, 0, 0, 0,
-            _nbytes(k_pool), _nbytes(v_pool), 0)
-        self._check(lib().pam_engine_qk_norm_rope(self._ctx, C.byref(r)))
-
-    def qk_norm_rope_backward(self, q, k, d_q_out, d_k_out, d_q, d_k, positions, layer: PagedLayerSpec, q_weight=None,
-                              k_weight=None, d_q_weight=None, d_k_weight=None, eps: float = 1e-6,
-                              rotary: RotarySpec = None, normalize: bool = True):
-        """Gradients of qk_norm_rope's outputs: d_q, d_k and the weights' (float32), all written
-        (pam_engine_qk_norm_rope_backward).  q and k are the forward's inputs."""
-        import torch
-        io, n, rot = self._norm_args(layer, q, positions, q_weight, k_weight, normalize, rotary)
-        self._device_args((torch.float32,), d_q_weight=d_q_weight, d_k_weight=d_k_weight)
-        for w in (d_q_weight, d_k_weight):
-            self._want(w is None or w.numel() == layer.head_dim, "weights have head_dim entries.")
-        H, K = layer.num_heads, layer.num_kv_heads
-        (qp, qs), (kp, ks) = self._rows("q", q, H, layer, n, io), self._rows("k", k, K, layer, n, io)
-        gq, gqs = self._rows("d_q_out", d_q_out, H, layer, n, io)
-        gk, gks = self._rows("d_k_out", d_k_out, K, layer, n, io)
-        dq, dqs = self._rows("d_q", d_q, H, layer, n, io)
-        dk, dks = self._rows("d_k", d_k, K, layer, n, io)
-        r = _lib.QkNormRopeBackwardRequest(
-            qp, kp, gq, gk, dq, dk, _ptr(q_weight), _ptr(k_weight), _ptr(d_q_weight), _ptr(d_k_weight),
-            _ptr(positions), qs, ks, gqs, gks, dqs, dks, n, layer.c(), rot, float(eps), bool(normalize))
-        self._check(lib().pam_engine_qk_norm_rope_backward(self._ctx, C.byref(r)))
-
-    def tree_attention(self, q, k_pool, v_pool, block_tables, context_lens, cu_queries, tree_mask, output,
-                       max_queries, layer: PagedLayerSpec, k_scale=None, v_scale=None):
-        """Attention of drafted trees over the cache (pam_engine_tree_attention): q and output [rows, heads,
-        head_dim], sequence s's rows cu_queries[s] .. cu_queries[s + 1] - 1 (at most max_queries), its drafted keys
-        and values in the pools from position context_lens[s] on.  tree_mask [rows, words] int64, or None for
-        chains."""
-        import torch
-        io, pool = {0: (torch.float32, torch.float32), 1: (torch.float16, torch.float16),
-                    2: (torch.float16, torch.uint8)}[int(layer.data_type)]
-        self._device_args((io,), q=q, output=output)
-        self._device_args((pool,), k_pool=k_pool, v_pool=v_pool)
-        self._device_args((torch.int32,), block_tables=block_tables, context_lens=context_lens, cu_queries=cu_queries)
-        self._device_args((torch.int64,), tree_mask=tree_mask)
-        n = context_lens.numel()
-        shape = (layer.num_heads, layer.head_dim)
-        self._want(q.dim() == 3 and tuple(q.shape[1:]) == shape and output.shape == q.shape,
-                   f"q and output are [rows, {shape[0]}, {shape[1]}].")
-        self._want(block_tables.dim() == 2 and block_tables.shape[0] == n and cu_queries.numel() == n + 1,
-                   f"block_tables and cu_queries need the {n} sequences of context_lens.")
-        self._want(tree_mask is None or (tree_mask.dim() == 2 and tree_mask.shape[0] == q.shape[0]),
-                   "tree_mask needs one row per query row.")
-        r = _lib.TreeAttentionRequest(
-            _ptr(q), _ptr(output), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables), _ptr(context_lens),
-            _ptr(cu_queries), _ptr(tree_mask), 0 if tree_mask is None else tree_mask.shape[1], n,
-            block_tables.shape[1], int(max_queries), q.shape[0], layer.c(), _ptr(k_scale), _ptr(v_scale), 0, 0,
-            _nbytes(k_pool), _nbytes(v_pool))
-        self._check(lib().pam_engine_tree_attention(self._ctx, C.byref(r)))
-
-    def tree_commit(self, k_pool, v_pool, block_tables, context_lens, query_lens, paths, layer: PagedLayerSpec,
-                    new_lengths=None, k_scale=None, v_scale=None):
-        """The accepted path of every sequence moved to the end of its cached tokens (pam_engine_tree_commit):
-        paths [sequences, at most] int32, a path's nodes in rising order, -1 behind them."""
-        import torch
-        pool = {0: torch.float32, 1: torch.float16, 2: torch.uint8}[int(layer.data_type)]
-        self._device_args((pool,), k_pool=k_pool, v_pool=v_pool)
-        self._device_args((torch.int32,), block_tables=block_tables, context_lens=context_lens,
-                          query_lens=query_lens, paths=paths, new_lengths=new_lengths)
-        n = context_lens.numel()
-        self._want(block_tables.dim() == 2 and block_tables.shape[0] == n and paths.dim() == 2 and
-                   paths.shape[0] == n and query_lens.numel() == n and
-                   (new_lengths is None or new_lengths.numel() == n),
-                   f"every argument needs the {n} sequences of context_lens.")
-        r = _lib.TreeCommitRequest(
-            _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), _ptr(context_lens),
-            _ptr(query_lens), _ptr(paths), _ptr(new_lengths), n, block_tables.shape[1], paths.shape[1], layer.c(),
-            _nbytes(k_pool), _nbytes(v_pool))
-        self._check(lib().pam_engine_tree_commit(self._ctx, C.byref(r)))
 
     # --- calibration streams (achievable HBM rates, counter scaling)
     def calib_stream_read(self, src, blocks=0) -> float:

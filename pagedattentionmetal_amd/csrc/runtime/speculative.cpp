@@ -53,12 +53,13 @@ void set_rotation(const pam_rotary_spec &r, const pam_layer_spec &l, NormRopePar
     need(r.rotary_dim == 0 || r.inv_freq || (r.base > 0.0 && std::isfinite(r.base)), "the rotation's base must be positive.");
     p.rotary_dim = r.rotary_dim;
     p.interleaved = r.interleaved ? 1 : 0;
-    const long double two_pi = 6.283185307179586476925286766559L;
+    const long double turn = 0.15915494309189533576888376337251L;  // 1 / 2 pi
     for (int32_t i = 0; i < r.rotary_dim / 2; i++) {
         const double f = r.inv_freq ? r.inv_freq[i] : std::pow(r.base, -2.0 * i / r.rotary_dim);
         need(std::isfinite(f), "the rotation's frequencies must be finite.");
-        const long double turns = (long double)f / two_pi, frac = turns - std::floor(turns);
-        const long double scaled = std::nearbyint(std::ldexp(frac, 64));
+        long double t = (long double)f * turn;
+        if (t < 0.0L || t >= 1.0L) t -= std::floor(t);
+        const long double scaled = t * 18446744073709551616.0L + 0.5L;
         p.freq[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
     }
 }

@@ -147,6 +147,35 @@ def test_rotary_spec():
             RotarySpec(**bad)
 
 
+@pytest.mark.parametrize("cls", [_lib.BatchPlanRequest, _lib.QkNormRopeRequest, _lib.QkNormRopeBackwardRequest,
+                                 _lib.TreeAttentionRequest, _lib.TreeCommitRequest])
+def test_packed_requests_are_the_structs_bytes(cls):
+    """Every field of its own value, packed and through the ctypes structure."""
+    values, r, n = [], cls(), 0
+
+    def fill(s):
+        nonlocal n
+        for name, t in s._fields_:
+            if issubclass(t, C.Structure):
+                fill(getattr(s, name))
+                continue
+            n += 1
+            v = True if t is C.c_bool else (n * 0.5 if t in (C.c_float, C.c_double) else n * 1000003)
+            setattr(s, name, v)
+            values.append(v)
+    fill(r)
+    got, ref = _lib.packer(cls)(*values), bytes(r)
+    assert len(got) == C.sizeof(cls)
+    back = cls.from_buffer_copy(got)
+
+    def same(a, b):
+        for name, t in a._fields_:
+            x, y = getattr(a, name), getattr(b, name)
+            assert same(x, y) if issubclass(t, C.Structure) else x == y, name
+        return True
+    assert same(r, back) and len(ref) == len(got)
+
+
 def test_host_tensors_and_wrong_types_are_refused():
     import torch
     e = PagedAttentionEngine()
