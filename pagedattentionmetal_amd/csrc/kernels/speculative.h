@@ -73,9 +73,8 @@ struct TreeParams {
     const uint64_t *tree_mask;    // [total_rows][mask_words] or null (chains)
     int32_t mask_words, num_seqs, max_queries, total_rows;
     int32_t pool_blocks;          // blocks of the pools: table entries are held below it
-    // the split (tree_plan): workgroups that share all units (UNIT keys of a block of
-    // block_rows query rows) equally, at least min_units each
-    int32_t form, block_rows, unit_keys, groups, min_units;
+    // the split (tree_plan): `groups` workgroups share all units equally
+    int32_t form, block_rows, rows_log2, keys_log2, groups;
 };
 enum TreeForm : int32_t { kTreeRow = 0, kTreeRowBlocks = 1, kTreeMfma = 2 };
 // Chooses the kernel and the split; returns the bytes of partials it needs (a.part_o,

@@ -1,16 +1,16 @@
 // tree_attention.hip - attention of drafted trees over a paged cache (gfx950): the kernels
 // and their choice.
 //   tree_mfma_kernel   f16 and e4m3 pools, head sizes up to 128 (tree_mfma.h)
-//   tree_rows_kernel   f32 pools and larger heads: f32 probabilities on the matrix units
+//   tree_rows_kernel   f32 pools, larger heads, odd blocks: f32 probabilities on the matrix units
 //                      (RowTiles, rows_body.h)
 //   tree_row_kernel    what has no whole 16-byte (e4m3: 8-byte) pieces
-// The first two share the chip by equal counts of units and leave partials that
-// tree_reduce_kernel merges (tree_body.h).
+// The first two share the chip by equal counts of units (tree_body.h).
 #include <algorithm>
 
 #include "tree_mfma.h"
 
 namespace pam {
+
 
 // ------------------------------------------------------------------ one row a workgroup
 // Any head size (a multiple of 4), group and alignment: a workgroup serves one (row,
@@ -95,34 +95,34 @@ struct TreeSee {
     __device__ __forceinline__ int lo_all(const TileKeys &) const { return all; }
 };
 
+constexpr int kTreeRowKeys = 16 * kRowsWaves;  // keys of a unit: a tile for every wave
+
 template <typename KV, typename QT, int NT, int RB>
 __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_kernel(TreeParams p) {
     typedef RowTiles<KV, QT, NT, RB> Tiles;
-    constexpr int LS = Tiles::LS, RN = 16 * RB;
+    constexpr int LS = Tiles::LS, RN = 16 * RB, KEYS = kTreeRowKeys;
     __shared__ __attribute__((aligned(16))) float lds[kRowsLds<NT, RB>];
     const AttnParams &a = p.a;
     const int wave = threadIdx.x >> 6, H = a.num_heads, G = H / a.num_kv_heads, d = a.head_dim;
-    const int64_t group = (blockIdx.x % kXcds) * (int64_t)(gridDim.x / kXcds) + blockIdx.x / kXcds;
-    const TreeWork w = tree_work(p);
-    int64_t u = group * w.per;
-    const int64_t end = u + w.per < w.units ? u + w.per : w.units;
-    if (u >= end) return;
+    TreeWork w;
     TreeItem it;
-    tree_find(p, u, it);
+    if (!tree_start(p, w, it)) return;
+    int u = w.group * w.per;
+    const int end = u + w.per < w.units ? u + w.per : w.units;
     for (;;) {
-        const int64_t item_end = it.first + it.tiles, u1 = item_end < end ? item_end : end;
-        const TreeRows tr = tree_rows(p, it, 16);
+        const int item_end = it.first + it.tiles, u1 = item_end < end ? item_end : end;
+        const TreeRows tr = tree_rows<16>(p, it);
         TileKeys keys;
         keys.bt = it.q.bt;
         keys.block_size = a.block_size;
         keys.shift = block_shift(a.block_size);
-        keys.key0 = (it.tile0 + (int)(u - it.first)) * p.unit_keys;
+        keys.key0 = (it.tile0 + u - it.first) * KEYS;
         keys.lo = tree_first_key(p, it.q);
         keys.hi = it.q.hi;
         keys.hi_all = it.q.c;
         const int64_t all = (int64_t)it.q.c + it.q.n - a.window;
         const int lo_all = a.window > 0 && all > 0 ? (int)(all < it.q.c ? all : it.q.c) : 0;
-        const int key_end = (it.tile0 + (int)(u1 - it.first)) * p.unit_keys;
+        const int key_end = (it.tile0 + u1 - it.first) * KEYS;
         const int ntiles = keys.hi > keys.lo ? ((key_end < keys.hi ? key_end : keys.hi) - keys.key0 + 15) / 16 : 0;
 
         Tiles x;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
             x.put(b, 1.0f, lds + (wave * RN + 16 * b + x.n) * LS);
         }
         __syncthreads();
-        tree_write<KV, QT, LS>(p, it, tr, w, group, u, u1, lds, (int64_t)RN * LS, ml, RN * 2, kRowsWaves, any_odd, lo_all);
+        tree_write<KV, QT, LS>(p, it, tr, w, u, u1, lds, RN * LS, ml, RN * 2, kRowsWaves, any_odd, lo_all);
         u = u1;
         if (u >= end) break;
         tree_next(p, it);
@@ -159,56 +159,104 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
 
 // ------------------------------------------------------------------ merge
 
-// The partials of the items that several workgroups share, in order.  grid: x = row block
-// and slice of its rows, y = kv head, z = sequence
-constexpr int kTreeReduceRows = 8;
+// The partials of the items that several workgroups share, in order.  grid: x = slice of
+// slice_rows rows of a row block, y = kv head, z = sequence.  A thread adds 4 dims of a row;
+// with `ways` > 1 so many threads share the row's partials.  What bounds it: few
+// partials, their bytes; else the latency of the lengths and the partials behind one another,
+// so a thread asks for 8 partials and their states at once.
+constexpr int kTreeReduceThreads = 512;
 template <typename QT>
-__global__ __launch_bounds__(256) void tree_reduce_kernel(TreeParams p) {
-    const int slices = (p.block_rows + kTreeReduceRows - 1) / kTreeReduceRows;
+__global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreeParams p, int slice_rows, int ways) {
+    __shared__ float sums[kTreeReduceThreads][6];
+    const int slices = ((1 << p.rows_log2) + slice_rows - 1) / slice_rows;
+    const int lane = threadIdx.x & 63;
     TreeItem it;
-    tree_enter(p, blockIdx.z, it);
-    it.rb = blockIdx.x / slices;
+    it.s = blockIdx.z;
     it.kvh = blockIdx.y;
-    if (it.rb >= it.blocks) return;
-    int64_t before = 0, t = 0;
-    for (int s = threadIdx.x & 63; s < p.num_seqs; s += 64) {
-        const int64_t v = tree_units(p, s);
-        t += v;
+    it.rb = blockIdx.x / slices;
+    int before = 0, sum = 0;
+    for (int s = lane; s < p.num_seqs; s += 64) {
+        TreeSeq q;
+        const int v = tree_units(p, s, q);
+        sum += v;
         before += s < it.s ? v : 0;
     }
+    it.q = tree_seq(p, it.s);
+    tree_shape(p, it);
+    if (it.rb >= it.blocks) return;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64), before += __shfl_xor(before, m, 64);
+    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64), before += __shfl_xor(before, m, 64);
     TreeWork w;
-    w.units = t;
-    w.per = (t + p.groups - 1) / p.groups;
-    if (w.per < p.min_units) w.per = p.min_units;
-    it.first = before + ((int64_t)it.kvh * it.blocks + it.rb) * it.tiles;
-    const int64_t g0 = it.first / w.per, g1 = (it.first + it.tiles - 1) / w.per;
-    if (g0 == g1) return;  // one workgroup wrote its rows
-    const TreeRows tr = tree_rows(p, it, p.form == kTreeMfma ? 32 : 16);
-    const int d = p.a.head_dim, pieces = d / 4, r0 = (int)(blockIdx.x % slices) * kTreeReduceRows;
-    const int rn = tr.rows - r0 < kTreeReduceRows ? tr.rows - r0 : kTreeReduceRows;
-    // slot of group g0 by where the item begins; those of the others are their first
-    const float *o0 = tree_part_o(p, tree_slot(w, g0, it.first)), *ml0 = tree_part_ml(p, tree_slot(w, g0, it.first));
-    const float *o1 = tree_part_o(p, 2 * (g0 + 1)), *ml1 = tree_part_ml(p, 2 * (g0 + 1));
-    const int64_t step = 2 * (int64_t)p.block_rows * (d + 2);
-    const int n = (int)(g1 - g0);
-    for (int i = threadIdx.x; i < rn * pieces; i += 256) {
-        const int r = r0 + i / pieces, e0 = i % pieces * 4;
-        float M = ml0[2 * r];
-        for (int k = 0; k < n; k++) M = fmaxf(M, ml1[k * step + 2 * r]);
-        const float mu = M == -INFINITY ? 0.0f : M;
-        const float w0 = exp2f(ml0[2 * r] - mu);
-        const float4 v0 = *reinterpret_cast<const float4 *>(o0 + (int64_t)r * d + e0);
-        TreeSum s{{w0 * v0.x, w0 * v0.y, w0 * v0.z, w0 * v0.w}, w0 * ml0[2 * r + 1], M};
-#pragma unroll 4
-        for (int k = 0; k < n; k++) {
-            const float wk = exp2f(ml1[k * step + 2 * r] - mu);
-            const float4 v = *reinterpret_cast<const float4 *>(o1 + k * step + (int64_t)r * d + e0);
-            s.den += wk * ml1[k * step + 2 * r + 1];
-            s.a[0] += wk * v.x, s.a[1] += wk * v.y, s.a[2] += wk * v.z, s.a[3] += wk * v.w;
+    tree_share(p, __builtin_amdgcn_readfirstlane(sum), w);
+    it.first = __builtin_amdgcn_readfirstlane(before) + (it.kvh * it.blocks + it.rb) * it.tiles;
+    const int g0 = (int)((uint32_t)it.first / (uint32_t)w.per);
+    const int np = (int)((uint32_t)(it.first + it.tiles - 1) / (uint32_t)w.per) - g0 + 1;
+    if (np == 1) return;  // one workgroup wrote its rows
+    const TreeRows tr = p.form == kTreeMfma ? tree_rows<32>(p, it) : tree_rows<16>(p, it);
+    const int d = p.a.head_dim, pieces = d / 4, r0 = (int)(blockIdx.x % slices) * slice_rows;
+    const int rn = tr.rows - r0 < slice_rows ? tr.rows - r0 : slice_rows;
+    const int share = kTreeReduceThreads / ways, way = threadIdx.x / share, me = threadIdx.x % share;
+    const float *first_part = tree_part(p, 2 * g0);
+    const int64_t stride = 2 * (int64_t)((d + 2) << p.rows_log2);  // a workgroup's two places
+    // rounds of equal length in all threads: the sums below meet at a barrier
+    for (int i0 = 0; i0 < rn * pieces; i0 += share) {
+        const int i = i0 + me, x = i / pieces, e0 = (i - x * pieces) * 4;
+        const bool on = x < rn;
+        TreeSum s{{0.f, 0.f, 0.f, 0.f}, 0.0f, -INFINITY};
+        for (int k0 = way; on && k0 < np; k0 += 8 * ways) {
+            float4 v[8];
+            float2 ml[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int k = k0 + j * ways;
+                ml[j] = make_float2(-INFINITY, 0.0f);
+                v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < np) {
+                    // tree_slot: the item is the second of its first workgroup only
+                    const float *part = first_part + k * stride;
+                    if (k == 0 && it.first > g0 * w.per) part += stride / 2;
+                    ml[j] = *reinterpret_cast<const float2 *>(part + (d << p.rows_log2) + 2 * (r0 + x));
+                    v[j] = *reinterpret_cast<const float4 *>(part + (r0 + x) * d + e0);
+                }
+            }
+            float top = s.M;
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, ml[j].x);
+            const float mu = top == -INFINITY ? 0.0f : top, old = exp2f(s.M - mu);
+            s.M = top;
+            s.den *= old;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s.a[e] *= old;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float wk = exp2f(ml[j].x - mu);
+                s.den += wk * ml[j].y;
+                s.a[0] += wk * v[j].x, s.a[1] += wk * v[j].y, s.a[2] += wk * v[j].z, s.a[3] += wk * v[j].w;
+            }
         }
-        tree_out<QT>(p, it, tr.row0 + r, e0, s);
+        if (ways > 1) {
+            float *mine = sums[threadIdx.x];
+#pragma unroll
+            for (int e = 0; e < 4; e++) mine[e] = s.a[e];
+            mine[4] = s.M, mine[5] = s.den;
+            __syncthreads();
+            if (way == 0) {
+                for (int k = 1; k < ways; k++) s.M = fmaxf(s.M, sums[k * share + me][4]);
+                const float mu = s.M == -INFINITY ? 0.0f : s.M, own = exp2f(mine[4] - mu);
+                s.den *= own;
+#pragma unroll
+                for (int e = 0; e < 4; e++) s.a[e] *= own;
+                for (int k = 1; k < ways; k++) {
+                    const float *o = sums[k * share + me];
+                    const float wk = exp2f(o[4] - mu);
+                    s.den += wk * o[5];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s.a[e] += wk * o[e];
+                }
+            }
+            __syncthreads();
+        }
+        if (on && way == 0) tree_out<QT>(p, it, tr.row0 + r0 + x, e0, s);
     }
 }
 
@@ -219,40 +267,85 @@ static int tree_dim_slot(int32_t head_dim) {
     return nt <= 4 ? nt - 1 : 4;
 }
 
+// workgroups of a CU and keys of a unit of the matrix kernel for `rows` query rows a block
+template <typename KV, int HD, int RW>
+static void tree_mfma_shape(int *per_cu, int *keys) {
+    *per_cu = TreeMfma<KV, HD, RW>::PER_CU;
+    *keys = TreeMfma<KV, HD, RW>::KEYS;
+}
+template <typename KV, int HD>
+static void tree_mfma_shape(int rows, int *per_cu, int *keys) {
+    switch (rows) {
+        case 32: tree_mfma_shape<KV, HD, 1>(per_cu, keys); break;
+        case 64: tree_mfma_shape<KV, HD, 2>(per_cu, keys); break;
+        case 128: tree_mfma_shape<KV, HD, 4>(per_cu, keys); break;
+        default:
+            if constexpr (sizeof(KV) == 1) tree_mfma_shape<KV, HD, 8>(per_cu, keys);
+            break;
+    }
+}
+
 int64_t tree_plan(TreeParams &p, int32_t dtype, int32_t cus) {
     const AttnParams &a = p.a;
     const int64_t G = a.num_heads / a.num_kv_heads, rows = (int64_t)p.max_queries * G;
     p.form = kTreeRow;
-    if (!rows_supported(a, dtype)) return 0;
-    const bool mfma = dtype != kF32 && a.head_dim <= 128;
-    p.form = mfma ? kTreeMfma : kTreeRowBlocks;
-    if (mfma) {
-        p.block_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : 128);
-        p.unit_keys = rows <= 32 ? 128 : 64;
+    if (!rows_supported(a, dtype) || rows >= ((int64_t)1 << 31) - 256) return 0;
+    int per_cu = 2, keys = kTreeRowKeys;
+    // a request of the matrix kernel takes 1 KB (64 pieces of 16 bytes) of the rows of one block
+    const int64_t elem = dtype == kFP8 ? 1 : 2, block = (int64_t)a.num_kv_heads * a.head_dim * elem * a.block_size;
+    if (dtype != kF32 && a.head_dim <= 128 && (a.block_size & (a.block_size - 1)) == 0 &&
+        (a.head_dim <= 64 ? 64 : 128) * elem * a.block_size >= 1024 && block < ((int64_t)1 << 31)) {
+        p.form = kTreeMfma;
+        // Blocks of 256 rows dequantise a key once for 256 rows, those of 128 twice, but a block with
+        // few rows leaves its waves idle, so they take what fills them: 4 sequences of 48000 tokens and
+        // 256 rows 308 us and 341; 16 of 128 - 4096 tokens and 64 - 256 rows (160 in the mean) 101 us
+        // and 82.  f16, with nothing to dequantise: 350 us and 358, 96 us and 76: 128 rows.
+        const int64_t mean = p.total_rows * G / std::max(p.num_seqs, 1);  // rows of a sequence
+        p.block_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 || dtype == kF16 || mean < 192 ? 128 : 256));
+        // the ring of codes takes whole 16-byte pieces of aligned rows
+        const uintptr_t pools = (uintptr_t)a.k_pool | (uintptr_t)a.v_pool;
+        if (dtype == kFP8 && p.block_rows > 64 && (a.head_dim % 16 != 0 || pools % 16 != 0)) p.block_rows = 64;
+        if (dtype == kF16)
+            a.head_dim <= 64 ? tree_mfma_shape<f16, 64>(p.block_rows, &per_cu, &keys)
+                             : tree_mfma_shape<f16, 128>(p.block_rows, &per_cu, &keys);
+        else
+            a.head_dim <= 64 ? tree_mfma_shape<uint8_t, 64>(p.block_rows, &per_cu, &keys)
+                             : tree_mfma_shape<uint8_t, 128>(p.block_rows, &per_cu, &keys);
     } else {
-        const bool one = rows <= 16 || (dtype == kF32 && a.head_dim > 128);
-        p.block_rows = one ? 16 : 32;
-        p.unit_keys = 16 * kRowsWaves;
+        p.form = kTreeRowBlocks;
+        p.block_rows = rows <= 16 || (dtype == kF32 && a.head_dim > 128) ? 16 : 32;
     }
-    // two workgroups a CU (a multiple of the XCDs), fewer when the batch can hold no more units
-    const int64_t tiles = ((int64_t)a.max_num_blocks * a.block_size + p.unit_keys - 1) / p.unit_keys + 1;
+    // the workgroups that fit the CUs (a multiple of the XCDs), fewer when the batch can hold no
+    // more units; a batch of more units than 31 bits count keeps the row kernel
+    const int64_t tiles = ((int64_t)a.max_num_blocks * a.block_size + keys - 1) / keys + 1;
     const int64_t most = (int64_t)p.num_seqs * a.num_kv_heads * ((rows + p.block_rows - 1) / p.block_rows) * tiles;
-    p.min_units = 1;
-    int64_t groups = std::min<int64_t>(2 * (int64_t)(cus > 0 ? cus : 1), most);
+    if (most >= (int64_t)1 << 30) {
+        p.form = kTreeRow;
+        return 0;
+    }
+    p.rows_log2 = __builtin_ctz((unsigned)p.block_rows);
+    p.keys_log2 = __builtin_ctz((unsigned)keys);
+    int64_t groups = std::min<int64_t>(per_cu * (int64_t)(cus > 0 ? cus : 1), most);
     groups = (groups + kXcds - 1) / kXcds * kXcds;
     p.groups = (int32_t)groups;
     return 2 * groups * p.block_rows * (a.head_dim + 2) * 4;
 }
 
+template <typename KV, int HD, int RW>
+static void launch_tree_mfma(const TreeParams &p, hipStream_t stream) {
+    hipLaunchKernelGGL((tree_mfma_kernel<KV, HD, RW>), dim3((unsigned)p.groups), dim3(64 * TreeMfma<KV, HD, RW>::WAVES), 0,
+                       stream, p);
+}
 template <typename KV, int HD>
 static void launch_tree_mfma(const TreeParams &p, hipStream_t stream) {
-    const dim3 grid((unsigned)p.groups), block(256);
-    if (p.block_rows == 32)
-        hipLaunchKernelGGL((tree_mfma_kernel<KV, HD, 1>), grid, block, 0, stream, p);
-    else if (p.block_rows == 64)
-        hipLaunchKernelGGL((tree_mfma_kernel<KV, HD, 2>), grid, block, 0, stream, p);
-    else
-        hipLaunchKernelGGL((tree_mfma_kernel<KV, HD, 4>), grid, block, 0, stream, p);
+    switch (p.block_rows) {
+        case 32: launch_tree_mfma<KV, HD, 1>(p, stream); break;
+        case 64: launch_tree_mfma<KV, HD, 2>(p, stream); break;
+        case 128: launch_tree_mfma<KV, HD, 4>(p, stream); break;
+        default:
+            if constexpr (sizeof(KV) == 1) launch_tree_mfma<KV, HD, 8>(p, stream);
+            break;
+    }
 }
 
 template <typename KV, typename QT, int NT>
@@ -278,11 +371,10 @@ hipError_t launch_tree_attention(const TreeParams &p, int32_t dtype, hipStream_t
     }
     if (p.a.part_o == nullptr || p.a.zero_page == nullptr) return hipErrorInvalidValue;
     if (p.form == kTreeMfma) {
-        if (dtype == kF16) {
+        if (dtype == kF16)
             p.a.head_dim <= 64 ? launch_tree_mfma<f16, 64>(p, stream) : launch_tree_mfma<f16, 128>(p, stream);
-        } else {
+        else
             p.a.head_dim <= 64 ? launch_tree_mfma<uint8_t, 64>(p, stream) : launch_tree_mfma<uint8_t, 128>(p, stream);
-        }
     } else if (dtype == kF32) {
         switch (tree_dim_slot(p.a.head_dim)) {
             case 0: launch_tree_rows<float, float, 1>(p, stream); break;
@@ -296,16 +388,21 @@ hipError_t launch_tree_attention(const TreeParams &p, int32_t dtype, hipStream_t
     } else {
         launch_tree_rows<uint8_t, f16, 8>(p, stream);
     }
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int G = p.a.num_heads / p.a.num_kv_heads;
-    const int blocks = (int)(((int64_t)p.max_queries * G + p.block_rows - 1) / p.block_rows);
-    const dim3 grid((unsigned)(blocks * ((p.block_rows + kTreeReduceRows - 1) / kTreeReduceRows)),
-                    (unsigned)p.a.num_kv_heads, (unsigned)p.num_seqs);
+    const int64_t G = p.a.num_heads / p.a.num_kv_heads, blocks = ((int64_t)p.max_queries * G + p.block_rows - 1) / p.block_rows;
+    // rows of a workgroup, by the batch's 16-row slices: a full chip takes many, so that few
+    // workgroups wait for the lengths (2048 slices: 13.7 us with 64 rows, 18.8 with 16); an idle one
+    // few, and 4 threads a row's piece (16 slices, 33 partials: 5.0 us, 7.0 with 16 rows; but 256
+    // slices: 11 us, 6 with 16 rows)
+    const int64_t slices = blocks * p.a.num_kv_heads * p.num_seqs * p.block_rows / 16;
+    const int slice_rows = slices <= 64 ? 4 : (slices <= 1024 ? 16 : 64), ways = slices <= 64 ? 4 : 1;
+    const dim3 grid((unsigned)(blocks * ((p.block_rows + slice_rows - 1) / slice_rows)), (unsigned)p.a.num_kv_heads,
+                    (unsigned)p.num_seqs);
     if (dtype == kF32)
-        hipLaunchKernelGGL(tree_reduce_kernel<float>, grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(tree_reduce_kernel<float>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways);
     else
-        hipLaunchKernelGGL(tree_reduce_kernel<f16>, grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(tree_reduce_kernel<f16>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways);
     return hipGetLastError();
 }
 

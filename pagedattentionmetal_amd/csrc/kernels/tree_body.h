@@ -6,6 +6,7 @@
 // the drafted tokens whose bits its mask has set; with a window W, the last W of the keys
 // it sees, in order of position.  A row that sees no key is zeros.
 #pragma once
+#include "prefill_body.h"
 #include "rows_body.h"
 #include "speculative.h"
 
@@ -115,85 +116,93 @@ __device__ __forceinline__ int tree_first_key(const TreeParams &p, const TreeSeq
 }
 
 // ------------------------------------------------------------------ the split
-// The work is cut into units: block_rows query rows (token, head) of one kv head and
-// unit_keys keys.  An item is a row block with all its keys; items lie one behind the other
+// The work is cut into units: a block of 2^rows_log2 query rows (token, head) of one kv head
+// and 2^keys_log2 keys.  An item is a row block with all its keys; items lie one behind the other
 // (sequence, kv head, block), and every workgroup takes the same number of units, wherever
 // items begin and end.  Lengths are known on the device alone, so each workgroup adds
-// them up itself (a wave at a time, 64 sequences a step).  An item that several workgroups
-// share leaves a partial each, which tree_reduce_kernel merges in order: no counters, no
-// atomics, the same bits every time.
+// them up itself (64 sequences a step).  Workgroups that share an item leave a partial each,
+// which tree_reduce_kernel merges in order.
 struct TreeWork {
-    int64_t units, per;  // all units, and units of a workgroup
+    int units, per, group;  // all units, units of a workgroup, this workgroup's place
 };
 struct TreeItem {
     TreeSeq q;
-    int s, kvh, rb;          // sequence, kv head, row block
-    int blocks, waves;       // row blocks of a kv head; 16- or 32-row parts of a block in use
-    int tile0, tiles;        // first key's unit and units of the item
-    int64_t first;           // its first unit
+    int s, kvh, rb;     // sequence, kv head, row block
+    int blocks;         // row blocks of a kv head
+    int tile0, tiles;   // first key's unit and units of the item
+    int first;          // its first unit
 };
 
 __device__ __forceinline__ int tree_row_blocks(const TreeParams &p, int n) {
-    const int64_t rows = (int64_t)n * (p.a.num_heads / p.a.num_kv_heads);
-    return (int)((rows + p.block_rows - 1) / p.block_rows);
+    return (n * (p.a.num_heads / p.a.num_kv_heads) + (1 << p.rows_log2) - 1) >> p.rows_log2;
 }
 __device__ __forceinline__ void tree_tiles(const TreeParams &p, const TreeSeq &q, int &tile0, int &tiles) {
-    tile0 = tree_first_key(p, q) / p.unit_keys;
-    tiles = (q.hi + p.unit_keys - 1) / p.unit_keys - tile0;
+    tile0 = tree_first_key(p, q) >> p.keys_log2;
+    tiles = ((q.hi + (1 << p.keys_log2) - 1) >> p.keys_log2) - tile0;
     if (tiles < 1) tiles = 1;  // a row without keys is written too
 }
-__device__ __forceinline__ int64_t tree_units(const TreeParams &p, int s) {
-    if (s >= p.num_seqs) return 0;
-    const TreeSeq q = tree_seq(p, s);
-    int tile0, tiles;
-    tree_tiles(p, q, tile0, tiles);
-    return (int64_t)tree_row_blocks(p, q.n) * p.a.num_kv_heads * tiles;
-}
-__device__ __forceinline__ TreeWork tree_work(const TreeParams &p) {
-    int64_t t = 0;
-    for (int s = threadIdx.x & 63; s < p.num_seqs; s += 64) t += tree_units(p, s);
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
-    TreeWork w;
-    w.units = t;
-    w.per = (t + p.groups - 1) / p.groups;
-    if (w.per < p.min_units) w.per = p.min_units;
-    return w;
-}
-__device__ __forceinline__ void tree_enter(const TreeParams &p, int s, TreeItem &it) {
-    it.s = s;
-    it.q = tree_seq(p, s);
+__device__ __forceinline__ void tree_shape(const TreeParams &p, TreeItem &it) {
     it.blocks = tree_row_blocks(p, it.q.n);
     tree_tiles(p, it.q, it.tile0, it.tiles);
 }
-// the item that holds unit u (u < units)
-__device__ __forceinline__ void tree_find(const TreeParams &p, int64_t u, TreeItem &it) {
+// units of sequence s (0 past the last)
+__device__ __forceinline__ int tree_units(const TreeParams &p, int s, TreeSeq &q) {
+    if (s >= p.num_seqs) return 0;
+    q = tree_seq(p, s);
+    int tile0, tiles;
+    tree_tiles(p, q, tile0, tiles);
+    return tree_row_blocks(p, q.n) * p.a.num_kv_heads * tiles;
+}
+__device__ __forceinline__ void tree_share(const TreeParams &p, int units, TreeWork &w) {
+    w.units = units;
+    w.per = (int)((uint32_t)(units + p.groups - 1) / (uint32_t)p.groups);
+}
+// This workgroup's share, and the item that holds its first unit (false: it has none)
+__device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, TreeItem &it) {
     const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    int s = 0;
-    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
-        const int64_t mine = tree_units(p, s0 + lane);
-        int64_t upto = mine;
+    // consecutive shares on one XCD: row blocks of a kv head read the same keys
+    w.group = (int)(blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds);
+    TreeSeq q{};
+    int mine = tree_units(p, lane, q), sum = mine;
+    for (int s = lane + 64; s < p.num_seqs; s += 64) {
+        TreeSeq other;
+        sum += tree_units(p, s, other);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+    tree_share(p, __builtin_amdgcn_readfirstlane(sum), w);
+    const int u = w.group * w.per;
+    if (u >= w.units) return false;
+    int base = 0, s0 = 0;
+    for (;;) {
+        int upto = mine;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
-            const int64_t o = __shfl_up(upto, m, 64);
+            const int o = __shfl_up(upto, m, 64);
             if (lane >= m) upto += o;
         }
         const uint64_t past = __ballot(base + upto > u);
         if (past) {
             const int at = __builtin_ctzll(past);
-            s = s0 + at;
-            base += __shfl(upto - mine, at, 64);
+            base += __builtin_amdgcn_readlane(upto - mine, at);
+            it.s = s0 + at;
+            it.q.c = __builtin_amdgcn_readlane(q.c, at);
+            it.q.n = __builtin_amdgcn_readlane(q.n, at);
+            it.q.hi = __builtin_amdgcn_readlane(q.hi, at);
+            it.q.row0 = __builtin_amdgcn_readlane(q.row0, at);
             break;
         }
-        base += __shfl(upto, 63, 64);
+        base += __builtin_amdgcn_readlane(upto, 63);
+        s0 += 64;
+        mine = tree_units(p, s0 + lane, q);
     }
-    s = __builtin_amdgcn_readfirstlane(s);
-    tree_enter(p, s, it);
-    const int64_t k = (u - base) / it.tiles;  // item of the sequence
-    it.kvh = (int)(k / it.blocks);
-    it.rb = (int)(k % it.blocks);
+    it.q.bt = p.a.block_tables + (int64_t)it.s * p.a.bt_stride;
+    tree_shape(p, it);
+    const int k = (int)((uint32_t)(u - base) / (uint32_t)it.tiles);  // item of the sequence
+    it.kvh = (int)((uint32_t)k / (uint32_t)it.blocks);
+    it.rb = k - it.kvh * it.blocks;
     it.first = base + k * it.tiles;
+    return true;
 }
 // the item behind it, when there is one
 __device__ __forceinline__ void tree_next(const TreeParams &p, TreeItem &it) {
@@ -203,32 +212,30 @@ __device__ __forceinline__ void tree_next(const TreeParams &p, TreeItem &it) {
     if (++it.kvh < p.a.num_kv_heads) return;
     it.kvh = 0;
     do {
-        if (it.s + 1 >= p.num_seqs) return;
-        tree_enter(p, it.s + 1, it);
+        if (++it.s >= p.num_seqs) return;
+        it.q = tree_seq(p, it.s);
+        tree_shape(p, it);
     } while (it.blocks == 0);
 }
-// rows of a block: the item's parts of `part` rows are dealt evenly over its blocks
+// The rows of a block, of the sequence's n G rows of the kv head: parts of PART rows are
+// dealt evenly over the item's blocks
 struct TreeRows {
-    int row0, rows;  // of the sequence's n G rows of the kv head
+    int row0, rows;
 };
-__device__ __forceinline__ TreeRows tree_rows(const TreeParams &p, const TreeItem &it, int part) {
+template <int PART>
+__device__ __forceinline__ TreeRows tree_rows(const TreeParams &p, const TreeItem &it) {
     const int n = it.q.n * (p.a.num_heads / p.a.num_kv_heads);
-    const int parts = (n + part - 1) / part, per = (parts + it.blocks - 1) / it.blocks * part;
+    const int parts = (n + PART - 1) / PART, per = (int)((uint32_t)(parts + it.blocks - 1) / (uint32_t)it.blocks) * PART;
     TreeRows r;
     r.row0 = it.rb * per;
     r.rows = n - r.row0 < per ? n - r.row0 : per;
     if (r.rows < 0) r.rows = 0;
     return r;
 }
-// the slot of workgroup w's partial of an item that begins at unit `first`
-__device__ __forceinline__ int64_t tree_slot(const TreeWork &w, int64_t group, int64_t first) {
+// A group leaves at most two partials: of the item that its share begins in, and of the one
+// that it ends in.
+__device__ __forceinline__ int tree_slot(const TreeWork &w, int group, int first) {
     return 2 * group + (first <= group * w.per ? 0 : 1);
-}
-__device__ __forceinline__ float *tree_part_o(const TreeParams &p, int64_t slot) {
-    return p.a.part_o + slot * p.block_rows * (p.a.head_dim + 2);
-}
-__device__ __forceinline__ float *tree_part_ml(const TreeParams &p, int64_t slot) {
-    return tree_part_o(p, slot) + (int64_t)p.block_rows * p.a.head_dim;
 }
 
 // 4 dims of a row from N states of it: O at o + i o_stride (unscaled, reference max m),
@@ -236,7 +243,7 @@ __device__ __forceinline__ float *tree_part_ml(const TreeParams &p, int64_t slot
 struct TreeSum {
     float a[4], den, M;
 };
-__device__ __forceinline__ TreeSum tree_sum(const float *o, int64_t o_stride, const float *ml, int64_t ml_stride, int n) {
+__device__ __forceinline__ TreeSum tree_sum(const float *o, int o_stride, const float *ml, int ml_stride, int n) {
     TreeSum s{{0.f, 0.f, 0.f, 0.f}, 0.0f, -INFINITY};
     for (int i = 0; i < n; i++) s.M = fmaxf(s.M, ml[i * ml_stride]);
     const float mu = s.M == -INFINITY ? 0.0f : s.M;
@@ -298,27 +305,29 @@ __device__ __forceinline__ void tree_odd(const TreeParams &p, const TreeItem &it
     }
 }
 
-// A workgroup's rows in LDS (`n` states a row) as outputs, or as the workgroup's partial
-// of an item that others share.
-template <typename KV, typename QT, int ROWS_STRIDE>
+__device__ __forceinline__ float *tree_part(const TreeParams &p, int slot) {
+    return p.a.part_o + (int64_t)slot * ((p.a.head_dim + 2) << p.rows_log2);  // [rows][d], then [rows] (m, l)
+}
+
+// A workgroup's rows in LDS (`states` a row: O at o, (m, l) at ml) as outputs, or as its
+// partial of an item that others share.  u0, u1: the units of the item that it did.
+template <typename KV, typename QT, int ROW_STRIDE>
 __device__ __forceinline__ void tree_write(const TreeParams &p, const TreeItem &it, const TreeRows &tr, const TreeWork &w,
-                                           int64_t group, int64_t u0, int64_t u1, const float *o, int64_t o_stride,
-                                           const float *ml, int64_t ml_stride, int states, bool any_odd, int lo_all) {
+                                           int u0, int u1, const float *o, int o_stride, const float *ml, int ml_stride,
+                                           int states, bool any_odd, int lo_all) {
     const int d = p.a.head_dim, pieces = d / 4;
     const bool whole = u0 == it.first && u1 == it.first + it.tiles;
-    const int64_t slot = tree_slot(w, group, u0);
-    float *po = tree_part_o(p, slot), *pml = tree_part_ml(p, slot);
-    const int j0 = (it.tile0 + (int)(u0 - it.first)) * p.unit_keys;
-    const int j1e = (it.tile0 + (int)(u1 - it.first)) * p.unit_keys, j1 = j1e < it.q.hi ? j1e : it.q.hi;
+    float *part = tree_part(p, tree_slot(w, w.group, u0)), *part_ml = part + (d << p.rows_log2);
+    const int j0 = (it.tile0 + u0 - it.first) << p.keys_log2, j1 = (it.tile0 + u1 - it.first) << p.keys_log2;
     for (int i = threadIdx.x; i < tr.rows * pieces; i += blockDim.x) {
         const int r = i / pieces, e0 = (i - r * pieces) * 4;
-        TreeSum s = tree_sum(o + r * ROWS_STRIDE + e0, o_stride, ml + r * 2, ml_stride, states);
-        if (any_odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1, lo_all, s);
+        TreeSum s = tree_sum(o + r * ROW_STRIDE + e0, o_stride, ml + r * 2, ml_stride, states);
+        if (any_odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1 < it.q.hi ? j1 : it.q.hi, lo_all, s);
         if (whole) {
             tree_out<QT>(p, it, tr.row0 + r, e0, s);
         } else {
-            store4<float>(po + (int64_t)r * d + e0, s.a);
-            if (e0 == 0) *reinterpret_cast<float2 *>(pml + 2 * r) = make_float2(s.M, s.den);
+            store4<float>(part + r * d + e0, s.a);
+            if (e0 == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(s.M, s.den);
         }
     }
 }

@@ -519,6 +519,105 @@ def test_tree_attention(dtype, ctx, new, H, K, d, bs, window, words, masks):
     assert eng.last_stats["operation"] == 11
 
 
+MORE_TREE_CASES = [
+    (2, [4000, 100], [64, 50], 8, 2, 128, 16, 0, 1, "tree"),                     # e4m3, blocks of 256 rows
+    (2, [900], [64], 8, 2, 64, 16, 0, 1, "any"),
+    (2, [250, 9], [64, 63], 8, 1, 96, 32, 70, 1, "tree"),
+    (2, [500, 30, 2], [64, 20, 7], 8, 2, 128, 16, 0, 1, "tree"),                 # of 128
+    (2, [333], [50], 8, 4, 64, 16, 0, 1, "any"),                                 # of 64, two of them
+    (2, [300], [40], 8, 2, 72, 16, 0, 1, "tree"),                                # heads of half pieces
+    (2, [300], [40], 8, 2, 128, 4, 0, 1, "tree"),                                # blocks below a request
+    (2, [300, 5], [40, 64], 8, 2, 256, 16, 0, 1, "tree"),
+    (2, [120], [33], 8, 2, 64, 8, 0, 1, "any"),
+    (1, [300, 5], [40, 64], 8, 2, 256, 16, 0, 1, "tree"),
+    (1, [120, 31], [33, 1], 8, 2, 128, 1, 0, 1, "tree"),
+    (1, [120, 31], [33, 64], 8, 2, 128, 4, 0, 1, "any"),
+    (1, [120, 31], [33, 64], 8, 2, 64, 8, 20, 1, "any"),
+    (1, [120], [64], 6, 2, 8, 64, 0, 1, "tree"),
+    (1, [200, 0], [300, 31], 4, 1, 64, 16, 0, 5, "tree"),
+    (0, [200, 0], [300, 31], 4, 1, 64, 16, 0, 5, "tree"),
+    (1, list(range(0, 70 * 13, 13)), [1 + i % 5 for i in range(70)], 4, 1, 128, 16, 0, 1, "tree"),   # past 64 sequences
+    (2, list(range(0, 130 * 7, 7)), [i % 4 for i in range(130)], 4, 1, 64, 16, 0, 1, "tree"),
+    (0, list(range(0, 70 * 5, 5)), [1 + i % 3 for i in range(70)], 2, 1, 32, 16, 0, 1, "chain"),
+]
+
+
+@pytest.mark.parametrize("dtype,ctx,new,H,K,d,bs,window,words,masks", MORE_TREE_CASES)
+def test_tree_attention_forms(dtype, ctx, new, H, K, d, bs, window, words, masks):
+    """A case for each block of rows, head size and block size that the kernels tell apart, and many sequences."""
+    b = Batch(np.random.default_rng(sum(ctx) + d + H + bs), dtype, ctx, new, H, K, d, bs, window, words, masks, spare=1)
+    b.check(b.run(_engine()))
+
+
+@pytest.mark.parametrize("dtype,d", [(2, 128), (1, 64), (0, 64)])
+def test_tree_attention_of_unaligned_pools(dtype, d):
+    """Pools that begin 4 elements inside an allocation (the least that the call takes), and e4m3 half a piece."""
+    import torch
+    from pagedattentionmetal_amd import PagedAttentionError
+    b = Batch(np.random.default_rng(12), dtype, [77, 150], [30, 12], 16, 4, d, 16, 0, 1, "tree")
+    host = (b.codes if dtype == 2 else (b.k, b.v))
+    ref, vmax, ds = b.exact()
+    for shift in (4, 8) if dtype == 2 else (4, 1):
+        pools = []
+        for x in host:
+            flat = torch.zeros(x.size + shift, dtype=to_dev(x).dtype, device="cuda")
+            flat[shift:] = to_dev(x).flatten()
+            pools.append(flat[shift:].view(x.shape))
+        ks, vs = (to_dev(x.view(np.uint16)) for x in b.scales) if dtype == 2 else (None, None)
+        q = to_dev(b.q)
+        out = torch.zeros_like(q)
+        args = (q, *pools, _i32(b.bt), _i32(b.ctx), _i32(b.cu), to_dev(b.mask.view(np.int64)), out, 30,
+                _layer(d, 16, 4, 16, dtype))
+        if shift == 1:
+            with pytest.raises(PagedAttentionError, match="aligned to 4 elements"):
+                _engine().tree_attention(*args, k_scale=ks, v_scale=vs)
+            continue
+        _engine().tree_attention(*args, k_scale=ks, v_scale=vs)
+        assert (np.abs(to_host(out).astype(np.float64) - ref) <= b.tolerance(ref, vmax, ds)).all()
+
+
+@pytest.mark.parametrize("dtype,nodes,bs", [(1, 8, 4), (1, 14, 4), (1, 32, 4), (2, 64, 8), (2, 32, 8)])
+def test_tree_attention_of_long_contexts(dtype, nodes, bs):
+    """300001 cached tokens of small blocks: a workgroup's share holds more blocks than it keeps the entries of.  A share
+    adds at most 300001 / 128 products of two keys to a sum, in f32, one behind the other, and its rounding counts for
+    numerator and denominator."""
+    import torch
+    H, K, d, ctx = 32, 8, 128, 300001
+    gen = torch.Generator(device="cuda").manual_seed(nodes)
+    L = ctx + nodes
+    nb = -(-L // bs)
+    G = H // K
+    bt = torch.randperm(nb, generator=gen, device="cuda").to(torch.int32).view(1, nb)
+    k, v = (torch.randn((nb, bs, K, d), generator=gen, device="cuda", dtype=torch.float16) for _ in range(2))
+    scales = None
+    pools = (k, v)
+    if dtype == 2:
+        scales = tuple((x.abs().amax((1, 2, 3)).float() / 448).half() for x in (k, v))
+        codes = tuple((x.float() / s.float()[:, None, None, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+                      for x, s in zip((k, v), scales))
+        k, v = (c.half() * s[:, None, None, None] for c, s in zip(codes, scales))
+        pools = tuple(c.view(torch.uint8) for c in codes)
+        scales = tuple(s.view(torch.uint16) for s in scales)
+    q = torch.randn((nodes, H, d), generator=gen, device="cuda", dtype=torch.float16)
+    on = _paths(_tree(np.random.default_rng(nodes), nodes))
+    out = torch.zeros_like(q)
+    _engine().tree_attention(q, *pools, bt, _i32([ctx]), _i32([0, nodes]), to_dev(_words(on, 1).view(np.int64)), out,
+                             nodes, _layer(d, H, K, bs, dtype), k_scale=scales and scales[0], v_scale=scales and scales[1])
+    hidden = torch.zeros((nodes, L), dtype=torch.bool, device="cuda")
+    hidden[:, ctx:] = torch.from_numpy(~on).cuda()
+    hidden = hidden.repeat_interleave(G, 0)
+    for kvh in range(K):
+        kk, vv = (x[bt[0].long(), :, kvh].reshape(nb * bs, d)[:L].double() for x in (k, v))
+        qh = q[:, kvh * G:(kvh + 1) * G].reshape(-1, d).double()
+        x = (qh @ kk.t().contiguous() / d ** 0.5).masked_fill_(hidden, -torch.inf)
+        ref = torch.softmax(x, -1) @ vv
+        ds = float((qh.abs() @ kk.abs().t().contiguous()).max()) / d ** 0.5
+        p = 2 * ((d / 4 + 12) * U * ds + 8 * U) + 2 * (ctx / 128) * U + 2 * HALF
+        tol = p * float(vv.abs().max()) + torch.clamp(ref.abs(), min=2.0 ** -14) * HALF
+        err = (out[:, kvh * G:(kvh + 1) * G].reshape(-1, d).double() - ref).abs()
+        assert bool((err <= tol).all()), (kvh, float((err / tol).max()))
+
+
 @pytest.mark.parametrize("dtype,d", [(1, 128), (1, 64), (1, 96), (0, 128), (0, 36), (1, 20)])
 def test_tree_attention_inf_and_nan_stay_with_the_rows_that_see_them(dtype, d):
     """Inf and NaN of drafted keys and values reach exactly the rows whose masks hold them; those of the cached context,
