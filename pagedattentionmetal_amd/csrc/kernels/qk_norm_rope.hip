@@ -57,7 +57,9 @@ struct RopeVec {
         Raw r;
 #pragma unroll
         for (int i = 0; i < V; i++) r[i] = (T)x[i];
-        *reinterpret_cast<Raw *>(p) = r;
+        // past the L2's lines: what stays dirty there is written back when the kernel ends, and the
+        // next waits for it (4133 f32 prompt tokens: 18.4 us, with plain stores 19.6)
+        __builtin_nontemporal_store(r, reinterpret_cast<Raw *>(p));
     }
 };
 template <typename T>
