@@ -586,7 +586,8 @@ int32_t pam_engine_qk_norm_rope_backward(void *context, const pam_qk_norm_rope_b
  * sees the cached tokens and the drafted tokens whose bits its row of tree_mask
  * ([total_rows][mask_words]) has set, NULL being a chain (tokens 0 .. i); with a window,
  * the last window_size of these keys, in order of position.  A row that sees no key is
- * zeros; rows behind the last sequence are left as they are.  f32, f16 and e4m3 pools. */
+ * zeros; rows behind the last sequence are left as they are.  output is not q.  f32, f16 and
+ * e4m3 pools. */
 typedef struct pam_tree_attention_request {
     const void *q;
     void *output;

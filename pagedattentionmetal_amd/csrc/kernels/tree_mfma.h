@@ -511,6 +511,8 @@ tree_mfma_kernel(TreeParams p) {
                         stage(t, b, g);
                         if (t + 1 < c1) fetch(t + 1, g);
                     } else if (t + 1 < c1) {
+                        // one wave has no barrier above: its own reads of the place are done
+                        if constexpr (RW == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         request(t + 1, b_next, lookup(t + 1));
                         tree_wait<RQ>();
                     } else {

@@ -30,15 +30,26 @@ void need(bool ok, const char *what) {
     if (!ok) throw invalid_configuration(what);
 }
 
+// products of request fields, which may be any
+int64_t times(int64_t a, int64_t b) {
+    int64_t r;
+    if (__builtin_mul_overflow(a, b, &r)) throw invalid_configuration("sizes overflow 64 bits.");
+    return r;
+}
+
 int32_t blocks_of(size_t k_bytes, size_t v_bytes, const pam_layer_spec &l) {
     need(k_bytes != 0 && v_bytes != 0, "the pools' sizes are needed.");
-    const int64_t block = pool_bytes_for(1, l), n = (int64_t)(std::min(k_bytes, v_bytes) / (size_t)block);
+    const int64_t block = times(l.block_size, kv_bytes_per_token(l)), n = (int64_t)(std::min(k_bytes, v_bytes) / (size_t)block);
     if (n < 1) throw buffer_too_small("K pool", block, (int64_t)std::min(k_bytes, v_bytes));
     return (int32_t)std::min<int64_t>(n, std::numeric_limits<int32_t>::max());
 }
 
 // bytes of rows `stride` elements apart, `row` elements used of each
-int64_t span(int64_t rows, int64_t stride, int64_t row, int32_t elem) { return ((rows - 1) * stride + row) * elem; }
+int64_t span(int64_t rows, int64_t stride, int64_t row, int32_t elem) {
+    // row <= stride: the sum fits when `rows` whole strides do
+    (void)times(times(rows, stride), elem);
+    return ((rows - 1) * stride + row) * elem;
+}
 
 int64_t stride_of(int64_t stride, int64_t row, const char *name) {
     if (stride == 0) return row;
@@ -264,6 +275,7 @@ void Context::tree_attention(const pam_tree_attention_request &r) {
     need(r.max_queries > 0, "maxQueries must be positive.");
     need(r.total_rows > 0, "totalRows must be positive.");
     need(r.num_seqs <= kMaxGridYZ && r.max_queries <= kMaxGridYZ, "at most 65535 sequences and queries of a sequence.");
+    need(l.num_kv_heads <= kMaxGridYZ, "at most 65535 key heads.");
     need((int64_t)r.max_num_blocks * l.block_size + r.max_queries <= std::numeric_limits<int32_t>::max() - 4096,
          "a sequence has at most 2^31 - 4096 tokens.");
     need(!r.tree_mask || (r.mask_words > 0 && r.max_queries <= 64 * (int64_t)r.mask_words),
@@ -276,14 +288,15 @@ void Context::tree_attention(const pam_tree_attention_request &r) {
     const uintptr_t kv = (uintptr_t)r.k_pool | (uintptr_t)r.v_pool, io = (uintptr_t)r.q | (uintptr_t)r.output;
     need(kv % (4 * elem_bytes(l.data_type)) == 0 && io % (4 * io_bytes(l.data_type)) == 0,
          "buffers must be aligned to 4 elements.");
-    require(r.q_bytes, "Q", r.total_rows * q_bytes_per_token(l));
-    require(r.output_bytes, "output", r.total_rows * q_bytes_per_token(l));
-    require(r.block_tables_bytes, "blockTables", (int64_t)r.num_seqs * r.max_num_blocks * 4);
+    require(r.q_bytes, "Q", times(r.total_rows, q_bytes_per_token(l)));
+    require(r.output_bytes, "output", times(r.total_rows, q_bytes_per_token(l)));
+    require(r.block_tables_bytes, "blockTables", times((int64_t)r.num_seqs * r.max_num_blocks, 4));
     require(r.context_lens_bytes, "contextLens", (int64_t)r.num_seqs * 4);
     require(r.cu_queries_bytes, "cuQueries", ((int64_t)r.num_seqs + 1) * 4);
-    if (r.tree_mask) require(r.tree_mask_bytes, "treeMask", (int64_t)r.total_rows * r.mask_words * 8);
+    if (r.tree_mask) require(r.tree_mask_bytes, "treeMask", times((int64_t)r.total_rows * r.mask_words, 8));
     TreeParams p{};
     p.pool_blocks = blocks_of(r.k_pool_bytes, r.v_pool_bytes, l);
+    need(r.output != r.q, "the output needs a buffer of its own.");
     ensure_device();
     const DeviceGuard guard(device_);
     const bool capturing = begin_spec();
@@ -336,10 +349,10 @@ void Context::tree_commit(const pam_tree_commit_request &r) {
     if (l.data_type == kFP8 && (!r.k_scale || !r.v_scale))
         throw invalid_configuration("FP8 tree commit needs the K and V scale pools.");
     need(((uintptr_t)r.k_pool | (uintptr_t)r.v_pool) % (l.data_type == kF16 ? 2 : 4) == 0, "pools must be aligned.");
-    require(r.block_tables_bytes, "blockTables", (int64_t)r.num_seqs * r.max_num_blocks * 4);
+    require(r.block_tables_bytes, "blockTables", times((int64_t)r.num_seqs * r.max_num_blocks, 4));
     require(r.context_lens_bytes, "contextLens", (int64_t)r.num_seqs * 4);
     require(r.query_lens_bytes, "queryLens", (int64_t)r.num_seqs * 4);
-    require(r.paths_bytes, "paths", (int64_t)r.num_seqs * r.max_path * 4);
+    require(r.paths_bytes, "paths", times((int64_t)r.num_seqs * r.max_path, 4));
     TreeCommitParams p{};
     p.pool_blocks = blocks_of(r.k_pool_bytes, r.v_pool_bytes, l);
     ensure_device();

@@ -139,8 +139,10 @@ class SpeculativeCalls:
         _want(len(width) == 2 and width[0] == n, "block_tables needs one row per sequence.")
         _want(slot_mapping.numel() == rows, "positions and slot_mapping need the same rows.")
         if tree_mask is not None:
-            _want(tree_mask.dim() == 2 and tree_mask.shape[0] == rows, "tree_mask needs one row per position.")
-            words = tree_mask.shape[1]
+            words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
+            _want(words > 0 and tree_mask.shape[0] == rows, "tree_mask needs one row per position.")
+        if parents is not None and parents.numel() == 0:
+            _want(False, "parents needs one entry per new token.")
         r = c.pack_batch_plan(
             _ptr(context_lens, i32, dev, "context_lens"), _ptr(query_lens, i32, dev, "query_lens"),
             _ptr(block_list, i32, dev, "block_list"), _ptr(parents, i32, dev, "parents"), block_list.numel(),
@@ -247,8 +249,8 @@ class SpeculativeCalls:
         _want(len(table) == 2 and table[0] == n and cu_queries.numel() == n + 1,
               "block_tables and cu_queries need the sequences of context_lens.")
         if tree_mask is not None:
-            _want(tree_mask.dim() == 2 and tree_mask.shape[0] == shape[0], "tree_mask needs one row per query row.")
-            words = tree_mask.shape[1]
+            words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
+            _want(words > 0 and tree_mask.shape[0] == shape[0], "tree_mask needs one row per query row.")
         kp, vp, ks, vs, kb, vb = self._pools(c, layer, dev, k_pool, v_pool, k_scale, v_scale)
         r = c.pack_tree_attention(
             _ptr(q, io, dev, "q"), _ptr(output, io, dev, "output"), kp, vp, _ptr(block_tables, i32, dev, "block_tables"),

@@ -1006,3 +1006,26 @@ def test_strict_code_object_and_injected_failures():
     e.set_module_strict(True)
     with pytest.raises(PagedAttentionError, match="not in the code object"):
         st.call(e)
+
+
+def test_empty_masks_and_parents_are_refused():
+    """A mask of no words and parents of no entries have no address, which elsewhere says that there are none."""
+    import torch
+    from pagedattentionmetal_amd import PagedAttentionError
+    eng = _engine()
+    i32, i64 = dict(dtype=torch.int32, device="cuda"), dict(dtype=torch.int64, device="cuda")
+    q = torch.zeros(2, 8, 64, dtype=torch.float16, device="cuda")
+    pool = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(PagedAttentionError, match="tree_mask needs one row"):
+        eng.tree_attention(q, pool, pool, torch.zeros(1, 4, **i32), torch.zeros(1, **i32), torch.zeros(2, **i32),
+                           torch.zeros(2, 0, **i64), torch.empty_like(q), 2, _layer(64, 8, 2))
+    with pytest.raises(PagedAttentionError, match="buffer of its own"):
+        eng.tree_attention(q, pool, pool, torch.zeros(1, 4, **i32), torch.zeros(1, **i32), torch.zeros(2, **i32),
+                           torch.zeros(2, 1, **i64), q, 2, _layer(64, 8, 2))
+    one = torch.zeros(1, **i32)
+    out = dict(cu_queries=torch.zeros(2, **i32), seq_lengths=torch.zeros(1, **i32), block_tables=torch.zeros(1, 4, **i32),
+               positions=torch.zeros(2, **i32), slot_mapping=torch.zeros(2, **i64))
+    with pytest.raises(PagedAttentionError, match="parents needs one entry"):
+        eng.batch_plan(one, one, one, 16, **out, parents=torch.zeros(0, **i32))
+    with pytest.raises(PagedAttentionError, match="tree_mask needs one row"):
+        eng.batch_plan(one, one, one, 16, **out, tree_mask=torch.zeros(2, 0, **i64))

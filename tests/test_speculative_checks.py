@@ -190,3 +190,29 @@ def test_host_tensors_and_wrong_types_are_refused():
         e.tree_attention(x, x, x, i.view(2, 1), i, i, None, x, 1, lay)
     with pytest.raises(PagedAttentionError, match="not on a GPU"):
         e.tree_commit(x, x, i.view(2, 1), i, i, i.view(2, 1), lay)
+
+
+BIG = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(), "the output needs a buffer of its own"),
+    (dict(output=FAKE + 4096, layer=dict(num_heads=1 << 17, num_kv_heads=1 << 16)), "at most 65535 key heads"),
+    (dict(layer=dict(num_heads=BIG // 2, num_kv_heads=1), total_rows=BIG, max_queries=64, num_seqs=1,
+          mask_words=1), "overflow"),
+    (dict(mask_words=BIG, total_rows=BIG), "overflow"),
+])
+def test_tree_attention_refuses_aliases_and_sizes_past_64_bits(change, text):
+    _refused("tree_attention", _tree(**change), text)
+
+
+def test_sizes_past_64_bits_are_refused():
+    """A block of 2^64 bytes, whose count of bytes wraps to zero, and rows whose ends do not fit."""
+    lay = _layer(block_size=1 << 30, num_heads=1 << 24, num_kv_heads=1 << 24, head_dim=256, data_type=0)
+    base = dict(k_pool=FAKE, v_pool=FAKE, block_tables=FAKE, context_lens=FAKE, query_lens=FAKE, paths=FAKE,
+                num_seqs=2, max_num_blocks=1, max_path=8, layer=lay, k_pool_bytes=1 << 20, v_pool_bytes=1 << 20)
+    _refused("tree_commit", _request(_lib.TreeCommitRequest, base), "overflow")
+    base.update(layer=_layer(block_size=1), num_seqs=BIG, max_num_blocks=BIG)
+    _refused("tree_commit", _request(_lib.TreeCommitRequest, base), "overflow")
+    _refused("qk_norm_rope", _norm(num_tokens=BIG, q_stride=1 << 40), "overflow")
+    _refused("qk_norm_rope", _norm(num_tokens=1, k_out_stride=(1 << 62) + 1), "overflow")
