@@ -160,8 +160,6 @@ __device__ __forceinline__ void tree_share(const TreeParams &p, int units, TreeW
 // This workgroup's share, and the item that holds its first unit (false: it has none)
 __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, TreeItem &it) {
     const int lane = threadIdx.x & 63;
-    // consecutive shares on one XCD: row blocks of a kv head read the same keys
-    w.group = (int)(blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds);
     TreeSeq q{};
     int mine = tree_units(p, lane, q), sum = mine;
     for (int s = lane + 64; s < p.num_seqs; s += 64) {
@@ -171,8 +169,13 @@ __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, Tre
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
     tree_share(p, __builtin_amdgcn_readfirstlane(sum), w);
+    // consecutive shares on one XCD, as row blocks of a kv head read the same keys, and as many
+    // shares on each
+    const int shares = (int)((uint32_t)(w.units + w.per - 1) / (uint32_t)w.per), of_xcd = (shares + kXcds - 1) / kXcds;
+    const int place = blockIdx.x / kXcds;
+    w.group = (int)(blockIdx.x % kXcds) * of_xcd + place;
     const int u = w.group * w.per;
-    if (u >= w.units) return false;
+    if (place >= of_xcd || u >= w.units) return false;
     int base = 0, s0 = 0;
     for (;;) {
         int upto = mine;
