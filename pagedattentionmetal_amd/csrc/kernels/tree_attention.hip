@@ -110,7 +110,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
     int u = w.group * w.per;
     const int end = u + w.per < w.units ? u + w.per : w.units;
     for (;;) {
-        const int item_end = it.first + it.tiles, u1 = item_end < end ? item_end : end;
+        const int u1 = tree_item_end(it, end);
         const TreeRows tr = tree_rows<16>(p, it);
         TileKeys keys;
         keys.bt = it.q.bt;
@@ -149,9 +149,10 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
             x.put(b, 1.0f, lds + (wave * RN + 16 * b + x.n) * LS);
         }
         __syncthreads();
-        tree_write<KV, QT, LS>(p, it, tr, w, u, u1, lds, RN * LS, ml, RN * 2, kRowsWaves, any_odd, lo_all);
+        tree_write<KV, QT, LS, 8 * NT, kRowsWaves, 64 * kRowsWaves>(p, it, tr, w, u, u1, lds, RN * LS, ml, RN * 2, any_odd,
+                                                                    lo_all);
         u = u1;
-        if (u >= end) break;
+        if (tree_last(w, u, end)) break;
         tree_next(p, it);
         __syncthreads();
     }
@@ -174,21 +175,18 @@ __global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreePar
     it.s = blockIdx.z;
     it.kvh = blockIdx.y;
     it.rb = blockIdx.x / slices;
-    int before = 0, sum = 0;
-    for (int s = lane; s < p.num_seqs; s += 64) {
-        TreeSeq q;
-        const int v = tree_units(p, s, q);
-        sum += v;
-        before += s < it.s ? v : 0;
-    }
+    TreeSeq own;
+    TreeWork w;
+    tree_share(p, tree_count(p, lane, own), w);
     it.q = tree_seq(p, it.s);
     tree_shape(p, it);
     if (it.rb >= it.blocks) return;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64), before += __shfl_xor(before, m, 64);
-    TreeWork w;
-    tree_share(p, __builtin_amdgcn_readfirstlane(sum), w);
-    it.first = __builtin_amdgcn_readfirstlane(before) + (it.kvh * it.blocks + it.rb) * it.tiles;
+    int before = 0;
+    for (int s = lane; s < it.s; s += 64) {
+        const TreeCount n = tree_count(p, s, own);
+        before += n.items * tree_padded(n.tiles, w.pad);
+    }
+    it.first = tree_wave_sum(before) + (it.kvh * it.blocks + it.rb) * tree_padded(it.tiles, w.pad);
     const int g0 = (int)((uint32_t)it.first / (uint32_t)w.per);
     const int np = (int)((uint32_t)(it.first + it.tiles - 1) / (uint32_t)w.per) - g0 + 1;
     if (np == 1) return;  // one workgroup wrote its rows

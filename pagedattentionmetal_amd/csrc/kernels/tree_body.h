@@ -118,12 +118,20 @@ __device__ __forceinline__ int tree_first_key(const TreeParams &p, const TreeSeq
 // ------------------------------------------------------------------ the split
 // The work is cut into units: a block of 2^rows_log2 query rows (token, head) of one kv head
 // and 2^keys_log2 keys.  An item is a row block with all its keys; items lie one behind the other
-// (sequence, kv head, block), and every workgroup takes the same number of units, wherever
-// items begin and end.  Lengths are known on the device alone, so each workgroup adds
-// them up itself (64 sequences a step).  Workgroups that share an item leave a partial each,
-// which tree_reduce_kernel merges in order.
+// (sequence, kv head, block), and every workgroup takes a share of `per` units.  Lengths are
+// known on the device alone, so each workgroup adds them up itself (64 sequences a step).
+// Workgroups that share an item leave a partial each, which tree_reduce_kernel merges in
+// order.
+//
+// Beginning and ending an item takes about 5 us, and its partial as many bytes as its rows,
+// so a share holds units of one item (items then begin at multiples of per: `pad`) where that
+// costs a workgroup at most a quarter and 4 more units.  One sequence of 4133 tokens, 264 units
+// on 256 workgroups: 18 us, and 22 when a share of 2 runs on into the next item; 16 ragged ones
+// (tree_mfma.h) 65 us and 72.  But 4 e4m3 sequences of 16384 to 65536 tokens, 150 units a
+// workgroup: 306 us with a quarter more, 281 with 4 at most.
 struct TreeWork {
     int units, per, group;  // all units, units of a workgroup, this workgroup's place
+    int pad;                // items begin at multiples of it
 };
 struct TreeItem {
     TreeSeq q;
@@ -145,30 +153,62 @@ __device__ __forceinline__ void tree_shape(const TreeParams &p, TreeItem &it) {
     it.blocks = tree_row_blocks(p, it.q.n);
     tree_tiles(p, it.q, it.tile0, it.tiles);
 }
-// units of sequence s (0 past the last)
-__device__ __forceinline__ int tree_units(const TreeParams &p, int s, TreeSeq &q) {
-    if (s >= p.num_seqs) return 0;
-    q = tree_seq(p, s);
-    int tile0, tiles;
-    tree_tiles(p, q, tile0, tiles);
-    return tree_row_blocks(p, q.n) * p.a.num_kv_heads * tiles;
+// shares of `per` units that an item fills
+__device__ __forceinline__ int tree_shares(int tiles, int per) {
+    return (int)(((uint32_t)tiles + (uint32_t)per - 1) / (uint32_t)per);
 }
-__device__ __forceinline__ void tree_share(const TreeParams &p, int units, TreeWork &w) {
-    w.units = units;
-    w.per = (int)((uint32_t)(units + p.groups - 1) / (uint32_t)p.groups);
+// units that an item takes, with those left empty behind it
+__device__ __forceinline__ int tree_padded(int tiles, int pad) { return tree_shares(tiles, pad) * pad; }
+// a sequence's items and units of one (no items past the last sequence)
+struct TreeCount {
+    int items, tiles;
+};
+__device__ __forceinline__ TreeCount tree_count(const TreeParams &p, int s, TreeSeq &q) {
+    if (s >= p.num_seqs) return {0, 0};
+    q = tree_seq(p, s);
+    TreeCount n;
+    int tile0;
+    tree_tiles(p, q, tile0, n.tiles);
+    n.items = tree_row_blocks(p, q.n) * p.a.num_kv_heads;
+    return n;
+}
+__device__ __forceinline__ int tree_wave_sum(int v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+// The split of the batch; `n`, `q`: the lane's own of the first 64 sequences
+__device__ __forceinline__ void tree_share(const TreeParams &p, const TreeCount &n, TreeWork &w) {
+    const int lane = threadIdx.x & 63;
+    auto shares = [&](int per) {  // at most as many as units
+        int sum = n.items * tree_shares(n.tiles, per);
+        for (int s = lane + 64; s < p.num_seqs; s += 64) {
+            TreeSeq q;
+            const TreeCount o = tree_count(p, s, q);
+            sum += o.items * tree_shares(o.tiles, per);
+        }
+        return tree_wave_sum(sum);
+    };
+    w.units = shares(1);
+    w.per = (int)((uint32_t)(w.units + p.groups - 1) / (uint32_t)p.groups);
+    w.pad = 1;
+    if (w.per <= 1) return;
+    const int more = w.per < 16 ? (w.per + 3) / 4 : 4;
+    for (int per = w.per; per <= w.per + more; per += more) {
+        const int used = shares(per);
+        if (used <= p.groups) {
+            w.units = used * per;
+            w.per = w.pad = per;
+            return;
+        }
+    }
 }
 // This workgroup's share, and the item that holds its first unit (false: it has none)
 __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, TreeItem &it) {
     const int lane = threadIdx.x & 63;
     TreeSeq q{};
-    int mine = tree_units(p, lane, q), sum = mine;
-    for (int s = lane + 64; s < p.num_seqs; s += 64) {
-        TreeSeq other;
-        sum += tree_units(p, s, other);
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-    tree_share(p, __builtin_amdgcn_readfirstlane(sum), w);
+    TreeCount n = tree_count(p, lane, q);
+    tree_share(p, n, w);
     // consecutive shares on one XCD, as row blocks of a kv head read the same keys, and as many
     // shares on each
     const int shares = (int)((uint32_t)(w.units + w.per - 1) / (uint32_t)w.per), of_xcd = (shares + kXcds - 1) / kXcds;
@@ -178,6 +218,7 @@ __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, Tre
     if (place >= of_xcd || u >= w.units) return false;
     int base = 0, s0 = 0;
     for (;;) {
+        const int mine = n.items * tree_padded(n.tiles, w.pad);
         int upto = mine;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
@@ -197,17 +238,24 @@ __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, Tre
         }
         base += __builtin_amdgcn_readlane(upto, 63);
         s0 += 64;
-        mine = tree_units(p, s0 + lane, q);
+        n = tree_count(p, s0 + lane, q);
     }
     it.q.bt = p.a.block_tables + (int64_t)it.s * p.a.bt_stride;
     tree_shape(p, it);
-    const int k = (int)((uint32_t)(u - base) / (uint32_t)it.tiles);  // item of the sequence
+    const int padded = tree_padded(it.tiles, w.pad);
+    const int k = (int)((uint32_t)(u - base) / (uint32_t)padded);  // item of the sequence
     it.kvh = (int)((uint32_t)k / (uint32_t)it.blocks);
     it.rb = k - it.kvh * it.blocks;
-    it.first = base + k * it.tiles;
+    it.first = base + k * padded;
     return true;
 }
-// the item behind it, when there is one
+// the end of the share's units of an item, and whether others follow in the share
+__device__ __forceinline__ int tree_item_end(const TreeItem &it, int end) {
+    const int item_end = it.first + it.tiles;
+    return item_end < end ? item_end : end;
+}
+__device__ __forceinline__ bool tree_last(const TreeWork &w, int u, int end) { return w.pad > 1 || u >= end; }
+// the item behind it, when there is one (items without padding)
 __device__ __forceinline__ void tree_next(const TreeParams &p, TreeItem &it) {
     it.first += it.tiles;
     if (++it.rb < it.blocks) return;
@@ -246,11 +294,14 @@ __device__ __forceinline__ int tree_slot(const TreeWork &w, int group, int first
 struct TreeSum {
     float a[4], den, M;
 };
-__device__ __forceinline__ TreeSum tree_sum(const float *o, int o_stride, const float *ml, int ml_stride, int n) {
+template <int N>
+__device__ __forceinline__ TreeSum tree_sum(const float *o, int o_stride, const float *ml, int ml_stride) {
     TreeSum s{{0.f, 0.f, 0.f, 0.f}, 0.0f, -INFINITY};
-    for (int i = 0; i < n; i++) s.M = fmaxf(s.M, ml[i * ml_stride]);
+#pragma unroll
+    for (int i = 0; i < N; i++) s.M = fmaxf(s.M, ml[i * ml_stride]);
     const float mu = s.M == -INFINITY ? 0.0f : s.M;
-    for (int i = 0; i < n; i++) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
         const float w = exp2f(ml[i * ml_stride] - mu);  // 0 for a state without keys
         const float4 v = *reinterpret_cast<const float4 *>(o + i * o_stride);
         s.den += w * ml[i * ml_stride + 1];
@@ -312,19 +363,22 @@ __device__ __forceinline__ float *tree_part(const TreeParams &p, int slot) {
     return p.a.part_o + (int64_t)slot * ((p.a.head_dim + 2) << p.rows_log2);  // [rows][d], then [rows] (m, l)
 }
 
-// A workgroup's rows in LDS (`states` a row: O at o, (m, l) at ml) as outputs, or as its
-// partial of an item that others share.  u0, u1: the units of the item that it did.
-template <typename KV, typename QT, int ROW_STRIDE>
+// A workgroup's rows in LDS (STATES a row: O at o, (m, l) at ml) as outputs, or as its
+// partial of an item that others share.  u0, u1: the units of the item that it did.  A row has
+// PIECES places for 4 dims.
+template <typename KV, typename QT, int ROW_STRIDE, int PIECES, int STATES, int THREADS>
 __device__ __forceinline__ void tree_write(const TreeParams &p, const TreeItem &it, const TreeRows &tr, const TreeWork &w,
                                            int u0, int u1, const float *o, int o_stride, const float *ml, int ml_stride,
-                                           int states, bool any_odd, int lo_all) {
-    const int d = p.a.head_dim, pieces = d / 4;
+                                           bool any_odd, int lo_all) {
+    const int d = p.a.head_dim;
     const bool whole = u0 == it.first && u1 == it.first + it.tiles;
     float *part = tree_part(p, tree_slot(w, w.group, u0)), *part_ml = part + (d << p.rows_log2);
     const int j0 = (it.tile0 + u0 - it.first) << p.keys_log2, j1 = (it.tile0 + u1 - it.first) << p.keys_log2;
-    for (int i = threadIdx.x; i < tr.rows * pieces; i += blockDim.x) {
-        const int r = i / pieces, e0 = (i - r * pieces) * 4;
-        TreeSum s = tree_sum(o + r * ROW_STRIDE + e0, o_stride, ml + r * 2, ml_stride, states);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < tr.rows * PIECES; i += THREADS) {
+        const int r = i / PIECES, e0 = (i - r * PIECES) * 4;
+        if (e0 >= d) continue;
+        TreeSum s = tree_sum<STATES>(o + r * ROW_STRIDE + e0, o_stride, ml + r * 2, ml_stride);
         if (any_odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1 < it.q.hi ? j1 : it.q.hi, lo_all, s);
         if (whole) {
             tree_out<QT>(p, it, tr.row0 + r, e0, s);

@@ -123,7 +123,7 @@ tree_mfma_kernel(TreeParams p) {
     const int k_rd = n * HD, k_sw = tree_k_swizzle<HD>(n);
 
     for (;;) {
-        const int item_end = it.first + it.tiles, u1 = item_end < end ? item_end : end;
+        const int u1 = tree_item_end(it, end);
         const TreeRows tr = tree_rows<32>(p, it);
         const TreeSeq &q = it.q;
         const int first = tree_first_key(p, q), hi = q.hi;
@@ -211,7 +211,7 @@ tree_mfma_kernel(TreeParams p) {
         auto clean = [&](int t, int buf) {
             if (full(t) || (RIN < RW && rw >= RIN) || (RQ == 1 && !(rw & 1))) return;
             f16 *vt = k_tile(buf) + TILE + lane * 8;
-#pragma unroll 1
+#pragma unroll 2
             for (int g = g0; g < g0 + NG; g++) {
                 f16x8 x = *reinterpret_cast<const f16x8 *>(vt + g * 512);
                 hide(key0(t, g) + my_row, x);
@@ -548,9 +548,10 @@ tree_mfma_kernel(TreeParams p) {
             if (h == 0) *reinterpret_cast<float2 *>(ml_lds + (wave * 32 + n) * 2) = make_float2(m_use, l);
         }
         __syncthreads();
-        tree_write<KV, f16, LS>(p, it, tr, w, u, u1, o_lds, RW * 32 * LS, ml_lds, RW * 64, KG, any_odd, lo_all);
+        tree_write<KV, f16, LS, HD / 4, KG, 64 * Shape::WAVES>(p, it, tr, w, u, u1, o_lds, RW * 32 * LS, ml_lds, RW * 64,
+                                                               any_odd, lo_all);
         u = u1;
-        if (u >= end) break;
+        if (tree_last(w, u, end)) break;
         tree_next(p, it);
         __syncthreads();
     }
