@@ -220,14 +220,14 @@ __global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreePar
             float top = s.M;
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, ml[j].x);
-            const float mu = top == -INFINITY ? 0.0f : top, old = exp2f(s.M - mu);
+            const float mu = top == -INFINITY ? 0.0f : top, old = __builtin_amdgcn_exp2f(s.M - mu);
             s.M = top;
             s.den *= old;
 #pragma unroll
             for (int e = 0; e < 4; e++) s.a[e] *= old;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float wk = exp2f(ml[j].x - mu);
+                const float wk = __builtin_amdgcn_exp2f(ml[j].x - mu);
                 s.den += wk * ml[j].y;
                 s.a[0] += wk * v[j].x, s.a[1] += wk * v[j].y, s.a[2] += wk * v[j].z, s.a[3] += wk * v[j].w;
             }
@@ -240,13 +240,13 @@ __global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreePar
             __syncthreads();
             if (way == 0) {
                 for (int k = 1; k < ways; k++) s.M = fmaxf(s.M, sums[k * share + me][4]);
-                const float mu = s.M == -INFINITY ? 0.0f : s.M, own = exp2f(mine[4] - mu);
+                const float mu = s.M == -INFINITY ? 0.0f : s.M, own = __builtin_amdgcn_exp2f(mine[4] - mu);
                 s.den *= own;
 #pragma unroll
                 for (int e = 0; e < 4; e++) s.a[e] *= own;
                 for (int k = 1; k < ways; k++) {
                     const float *o = sums[k * share + me];
-                    const float wk = exp2f(o[4] - mu);
+                    const float wk = __builtin_amdgcn_exp2f(o[4] - mu);
                     s.den += wk * o[5];
 #pragma unroll
                     for (int e = 0; e < 4; e++) s.a[e] += wk * o[e];

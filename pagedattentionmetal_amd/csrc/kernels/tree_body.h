@@ -172,11 +172,18 @@ __device__ __forceinline__ TreeCount tree_count(const TreeParams &p, int s, Tree
     n.items = tree_row_blocks(p, q.n) * p.a.num_kv_heads;
     return n;
 }
-__device__ __forceinline__ int tree_wave_sum(int v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    return __builtin_amdgcn_readfirstlane(v);
+// Sums over the lanes up to each: DPP moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31), as a
+// chain of 6 shuffles through LDS takes 0.35 us and a workgroup needs three
+__device__ __forceinline__ int tree_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
 }
+__device__ __forceinline__ int tree_wave_sum(int v) { return __builtin_amdgcn_readlane(tree_scan(v), 63); }
 // The split of the batch; `n`, `q`: the lane's own of the first 64 sequences
 __device__ __forceinline__ void tree_share(const TreeParams &p, const TreeCount &n, TreeWork &w) {
     const int lane = threadIdx.x & 63;
@@ -219,12 +226,7 @@ __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, Tre
     int base = 0, s0 = 0;
     for (;;) {
         const int mine = n.items * tree_padded(n.tiles, w.pad);
-        int upto = mine;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int o = __shfl_up(upto, m, 64);
-            if (lane >= m) upto += o;
-        }
+        const int upto = tree_scan(mine);
         const uint64_t past = __ballot(base + upto > u);
         if (past) {
             const int at = __builtin_ctzll(past);
@@ -302,7 +304,7 @@ __device__ __forceinline__ TreeSum tree_sum(const float *o, int o_stride, const 
     const float mu = s.M == -INFINITY ? 0.0f : s.M;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const float w = exp2f(ml[i * ml_stride] - mu);  // 0 for a state without keys
+        const float w = __builtin_amdgcn_exp2f(ml[i * ml_stride] - mu);  // 0 for a state without keys
         const float4 v = *reinterpret_cast<const float4 *>(o + i * o_stride);
         s.den += w * ml[i * ml_stride + 1];
         s.a[0] += w * v.x, s.a[1] += w * v.y, s.a[2] += w * v.z, s.a[3] += w * v.w;
@@ -311,11 +313,11 @@ __device__ __forceinline__ TreeSum tree_sum(const float *o, int o_stride, const 
 }
 template <typename QT>
 __device__ __forceinline__ void tree_out(const TreeParams &p, const TreeItem &it, int row, int e0, TreeSum &s) {
-    const int H = p.a.num_heads, G = H / p.a.num_kv_heads;
+    const int H = p.a.num_heads, G = H / p.a.num_kv_heads, node = (int)((uint32_t)row / (uint32_t)G);
     const float inv = s.den == 0.0f ? 0.0f : 1.0f / s.den;
 #pragma unroll
     for (int e = 0; e < 4; e++) s.a[e] *= inv;
-    const int64_t at = ((int64_t)(it.q.row0 + row / G) * H + it.kvh * G + row % G) * p.a.head_dim + e0;
+    const int64_t at = ((int64_t)(it.q.row0 + node) * H + it.kvh * G + (row - node * G)) * p.a.head_dim + e0;
     store4<QT>(static_cast<QT *>(p.a.out) + at, s.a);
 }
 
