@@ -102,6 +102,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
     typedef RowTiles<KV, QT, NT, RB> Tiles;
     constexpr int LS = Tiles::LS, RN = 16 * RB, KEYS = kTreeRowKeys;
     __shared__ __attribute__((aligned(16))) float lds[kRowsLds<NT, RB>];
+    __shared__ int odd_lds[kRowsWaves];
     const AttnParams &a = p.a;
     const int wave = threadIdx.x >> 6, H = a.num_heads, G = H / a.num_kv_heads, d = a.head_dim;
     TreeWork w;
@@ -139,7 +140,8 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
         x.run(a, keys, see, wave, ntiles, kRowsWaves);
 
         float *ml = lds + kRowsWaves * RN * LS;
-        const bool any_odd = __syncthreads_or(x.odd);
+        const bool wave_odd = __any(x.odd);
+        if ((threadIdx.x & 63) == 0) odd_lds[wave] = wave_odd;
 #pragma unroll
         for (int b = 0; b < RB; b++) {
             if (x.g == 0) {
@@ -149,6 +151,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
             x.put(b, 1.0f, lds + (wave * RN + 16 * b + x.n) * LS);
         }
         __syncthreads();
+        const bool any_odd = tree_any<kRowsWaves>(odd_lds);
         tree_write<KV, QT, LS, 8 * NT, kRowsWaves, 64 * kRowsWaves>(p, it, tr, w, u, u1, lds, RN * LS, ml, RN * 2, any_odd,
                                                                     lo_all);
         u = u1;

@@ -365,6 +365,16 @@ __device__ __forceinline__ float *tree_part(const TreeParams &p, int slot) {
     return p.a.part_o + (int64_t)slot * ((p.a.head_dim + 2) << p.rows_log2);  // [rows][d], then [rows] (m, l)
 }
 
+// Whether some wave left an element out: `flags`, written before a barrier by each wave (no LDS
+// clear, and two barriers fewer than __syncthreads_or)
+template <int WAVES>
+__device__ __forceinline__ bool tree_any(const int *flags) {
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) any |= flags[w];
+    return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+
 // A workgroup's rows in LDS (STATES a row: O at o, (m, l) at ml) as outputs, or as its
 // partial of an item that others share.  u0, u1: the units of the item that it did.  A row has
 // PIECES places for 4 dims.
@@ -376,18 +386,24 @@ __device__ __forceinline__ void tree_write(const TreeParams &p, const TreeItem &
     const bool whole = u0 == it.first && u1 == it.first + it.tiles;
     float *part = tree_part(p, tree_slot(w, w.group, u0)), *part_ml = part + (d << p.rows_log2);
     const int j0 = (it.tile0 + u0 - it.first) << p.keys_log2, j1 = (it.tile0 + u1 - it.first) << p.keys_log2;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < tr.rows * PIECES; i += THREADS) {
+    auto put = [&](int i, bool odd) {
         const int r = i / PIECES, e0 = (i - r * PIECES) * 4;
-        if (e0 >= d) continue;
+        if (e0 >= d) return;
         TreeSum s = tree_sum<STATES>(o + r * ROW_STRIDE + e0, o_stride, ml + r * 2, ml_stride);
-        if (any_odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1 < it.q.hi ? j1 : it.q.hi, lo_all, s);
+        if (odd) tree_odd<KV, QT>(p, it, tr.row0 + r, e0, j0, j1 < it.q.hi ? j1 : it.q.hi, lo_all, s);
         if (whole) {
             tree_out<QT>(p, it, tr.row0 + r, e0, s);
         } else {
             store4<float>(part + r * d + e0, s.a);
             if (e0 == 0) *reinterpret_cast<float2 *>(part_ml + 2 * r) = make_float2(s.M, s.den);
         }
+    };
+    if (!any_odd) {
+#pragma unroll 2
+        for (int i = threadIdx.x; i < tr.rows * PIECES; i += THREADS) put(i, false);
+    } else {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < tr.rows * PIECES; i += THREADS) put(i, true);
     }
 }
 

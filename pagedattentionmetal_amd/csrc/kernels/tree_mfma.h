@@ -86,6 +86,7 @@ tree_mfma_kernel(TreeParams p) {
     constexpr int PIECE = DMA ? 16 : 8, PIECES = HD * (int)sizeof(KV) / PIECE, RPR = 64 / PIECES;
     constexpr int RIN = 2 * 32 / RPR, RQ = RIN / RW > 0 ? RIN / RW : 1, NG = RQ / 2 > 0 ? RQ / 2 : 1;
     __shared__ __attribute__((aligned(16))) char smem[Shape::LDS];
+    __shared__ int odd_lds[Shape::WAVES];
     f16 *ring = reinterpret_cast<f16 *>(smem);
     uint8_t *raw = reinterpret_cast<uint8_t *>(smem + Shape::RING);
     int32_t *bt_lds = reinterpret_cast<int32_t *>(smem + Shape::RING + Shape::RAW);  // FP8: {block, K and V scale}
@@ -534,7 +535,7 @@ tree_mfma_kernel(TreeParams p) {
         }
 
         // the waves' rows in LDS, row-major, then out
-        const bool any_odd = __syncthreads_or(odd);
+        __syncthreads();
         {
             const float l = l_run + shfl_xor(l_run, 32);
             float *row = o_lds + (wave * 32 + n) * LS;
@@ -546,8 +547,11 @@ tree_mfma_kernel(TreeParams p) {
                     *reinterpret_cast<f32x4 *>(row + 32 * dt + 8 * r + 4 * h) = x;
                 }
             if (h == 0) *reinterpret_cast<float2 *>(ml_lds + (wave * 32 + n) * 2) = make_float2(m_use, l);
+            const bool wave_odd = __any(odd);
+            if (lane == 0) odd_lds[wave] = wave_odd;
         }
         __syncthreads();
+        const bool any_odd = tree_any<Shape::WAVES>(odd_lds);
         tree_write<KV, f16, LS, HD / 4, KG, 64 * Shape::WAVES>(p, it, tr, w, u, u1, o_lds, RW * 32 * LS, ml_lds, RW * 64,
                                                                any_odd, lo_all);
         u = u1;
