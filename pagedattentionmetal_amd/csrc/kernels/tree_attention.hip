@@ -1,10 +1,11 @@
 // tree_attention.hip - attention of drafted trees over a paged cache (gfx950): the kernels
 // and their choice.
 //   tree_mfma_kernel   f16 and e4m3 pools, head sizes up to 128 (tree_mfma.h)
-//   tree_rows_kernel   f32 pools, larger heads, odd blocks: f32 probabilities on the matrix units
-//                      (RowTiles, rows_body.h)
+//   tree_rows_kernel   f32 pools, larger heads, odd or small blocks: f32 probabilities on the
+//                      matrix units (RowTiles, rows_body.h)
 //   tree_row_kernel    what has no whole 16-byte (e4m3: 8-byte) pieces
-// The first two share the chip by equal counts of units (tree_body.h).
+// The first two share the chip by equal counts of units (tree_body.h) and tree_reduce_kernel
+// merges what they leave.
 #include <algorithm>
 
 #include "tree_mfma.h"
@@ -298,9 +299,10 @@ int64_t tree_plan(TreeParams &p, int32_t dtype, int32_t cus) {
         (a.head_dim <= 64 ? 64 : 128) * elem * a.block_size >= 1024 && block < ((int64_t)1 << 31)) {
         p.form = kTreeMfma;
         // Blocks of 256 rows dequantise a key once for 256 rows, those of 128 twice, but a block with
-        // few rows leaves its waves idle, so they take what fills them: 4 sequences of 48000 tokens and
-        // 256 rows 308 us and 341; 16 of 128 - 4096 tokens and 64 - 256 rows (160 in the mean) 101 us
-        // and 82.  f16, with nothing to dequantise: 350 us and 358, 96 us and 76: 128 rows.
+        // few rows leaves its waves idle, so only sequences that fill three quarters of one take it
+        // (e4m3, 4 sequences of 48000 tokens and 256 rows: 331 us and 354; 16 of 128 to 4096 tokens and
+        // 64 to 256 rows, 160 in the mean: 93 us and 72).  f16 has nothing to dequantise: blocks of 256
+        // rows took 350 us and 358 there, and 96 us and 76, so it has none.
         const int64_t mean = p.total_rows * G / std::max(p.num_seqs, 1);  // rows of a sequence
         p.block_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 || dtype == kF16 || mean < 192 ? 128 : 256));
         // the ring of codes takes whole 16-byte pieces of aligned rows

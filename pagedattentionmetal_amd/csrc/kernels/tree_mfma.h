@@ -20,10 +20,13 @@
 // 64-bit products in every lane cost 30% of the vector unit's time (f16, 16384 tokens and 256
 // rows: 455 us with them, 420 without).
 //
-// What bounds it (16 sequences, 32 heads on 8, head 128, both passes): few rows, memory (f16, 16384
-// tokens: 8 nodes 216 us, 5.0 TB/s; e4m3 130 us, 4.2 TB/s); many, the matrix and the vector
-// units, which take turns more than they overlap (f16, 64 nodes: 413 us, 0.66 PFLOP/s; the
-// softmax's exponentials alone take as long as half the products).
+// What bounds it (16 sequences, 32 heads on 8, head 128, with the merge): few rows, memory (f16,
+// 16384 tokens: 8 nodes 205 us, 5.3 TB/s of KV; 32 nodes 239 us, 4.5 TB/s; e4m3, 8 nodes 129 us,
+// 4.2 TB/s); many, the matrix and the vector units, which take turns more than they overlap (f16,
+// 64 nodes: 412 us, 0.67 PFLOP/s, matrix units busy a third of the time; the softmax's exponentials
+// alone take half as long as the products); one short sequence, latency: 12 us of a 4133-token
+// call are the lengths, the table's entries, the tiles, the merge of key groups and the store, one
+// behind the other.
 #pragma once
 #include "tree_body.h"
 
