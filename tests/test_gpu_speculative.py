@@ -549,6 +549,14 @@ def test_tree_attention_forms(dtype, ctx, new, H, K, d, bs, window, words, masks
     b.check(b.run(_engine()))
 
 
+@pytest.mark.parametrize("ctx,new,d,bs", [([700, 9], [64, 40], 64, 8), ([700, 9], [64, 40], 128, 4),
+                                          ([90], [20], 48, 4), ([90], [20], 64, 2), ([200], [4], 64, 8)])
+def test_tree_attention_of_small_e4m3_blocks(ctx, new, d, bs):
+    """Blocks that hold 64 pieces of 8 bytes of a head but not of 16, and fewer."""
+    b = Batch(np.random.default_rng(d + bs), 2, ctx, new, 8, 2, d, bs, 0, 1, "tree", spare=1)
+    b.check(b.run(_engine()))
+
+
 @pytest.mark.parametrize("dtype,d", [(2, 128), (1, 64), (0, 64)])
 def test_tree_attention_of_unaligned_pools(dtype, d):
     """Pools that begin 4 elements inside an allocation (the least that the call takes), and e4m3 half a piece."""
