@@ -170,32 +170,43 @@ __global__ __launch_bounds__(64 * kRowsWaves, (NT <= 4 ? 2 : 1)) void tree_rows_
 // ------------------------------------------------------------------ merge
 
 // The partials of the items that several workgroups share, in order.  grid: x = slice of
-// slice_rows rows of a row block, y = kv head, z = sequence.  A thread adds 4 dims of a row;
+// slice_rows rows of a row block, y = kv head, z = sequence; or, by_share, x = slice and share
+// boundary, for a batch with more items than shares, few of which are split (166 sequences, 8 kv
+// heads: 20 us, by item 36).  A thread adds 4 dims of a row;
 // with `ways` > 1 so many threads share the row's partials.  What bounds it: few
 // partials, their bytes; else the latency of the lengths and the partials behind one another,
 // so a thread asks for 8 partials and their states at once.
 constexpr int kTreeReduceThreads = 512;
 template <typename QT>
-__global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreeParams p, int slice_rows, int ways) {
+__global__ __launch_bounds__(kTreeReduceThreads) void tree_reduce_kernel(TreeParams p, int slice_rows, int ways, bool by_share) {
     __shared__ float sums[kTreeReduceThreads][6];
     const int slices = ((1 << p.rows_log2) + slice_rows - 1) / slice_rows;
     const int lane = threadIdx.x & 63;
     TreeItem it;
-    it.s = blockIdx.z;
-    it.kvh = blockIdx.y;
-    it.rb = blockIdx.x / slices;
-    TreeSeq own;
+    TreeSeq own{};
     TreeWork w;
-    tree_share(p, tree_count(p, lane, own), w);
-    it.q = tree_seq(p, it.s);
-    tree_shape(p, it);
-    if (it.rb >= it.blocks) return;
-    int before = 0;
-    for (int s = lane; s < it.s; s += 64) {
-        const TreeCount n = tree_count(p, s, own);
-        before += n.items * tree_padded(n.tiles, w.pad);
+    const TreeCount mine = tree_count(p, lane, own);
+    tree_share(p, mine, w);
+    if (by_share) {
+        // the item that the boundary cuts, if no boundary before cuts it
+        const int g = (int)(blockIdx.x / slices) + 1, u = g * w.per;
+        if (u >= w.units) return;
+        tree_find(p, w, u, mine, own, it);
+        if (it.first == u || it.first < (g - 1) * w.per) return;
+    } else {
+        it.s = blockIdx.z;
+        it.kvh = blockIdx.y;
+        it.rb = blockIdx.x / slices;
+        it.q = tree_seq(p, it.s);
+        tree_shape(p, it);
+        if (it.rb >= it.blocks) return;
+        int before = 0;
+        for (int s = lane; s < it.s; s += 64) {
+            const TreeCount n = tree_count(p, s, own);
+            before += n.items * tree_padded(n.tiles, w.pad);
+        }
+        it.first = tree_wave_sum(before) + (it.kvh * it.blocks + it.rb) * tree_padded(it.tiles, w.pad);
     }
-    it.first = tree_wave_sum(before) + (it.kvh * it.blocks + it.rb) * tree_padded(it.tiles, w.pad);
     const int g0 = (int)((uint32_t)it.first / (uint32_t)w.per);
     const int np = (int)((uint32_t)(it.first + it.tiles - 1) / (uint32_t)w.per) - g0 + 1;
     if (np == 1) return;  // one workgroup wrote its rows
@@ -404,18 +415,21 @@ hipError_t launch_tree_attention(const TreeParams &p, int32_t dtype, hipStream_t
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t G = p.a.num_heads / p.a.num_kv_heads, blocks = ((int64_t)p.max_queries * G + p.block_rows - 1) / p.block_rows;
+    const int64_t items = blocks * p.a.num_kv_heads * p.num_seqs;  // at most
+    const bool by_share = items > p.groups;
     // rows of a workgroup, by the batch's 16-row slices: a full chip takes many, so that few
     // workgroups wait for the lengths (2048 slices: 13.7 us with 64 rows, 18.8 with 16); an idle one
     // few, and 4 threads a row's piece (16 slices, 33 partials: 5.0 us, 7.0 with 16 rows; but 256
     // slices: 11 us, 6 with 16 rows)
-    const int64_t slices = blocks * p.a.num_kv_heads * p.num_seqs * p.block_rows / 16;
+    const int64_t slices = (by_share ? p.groups : items) * p.block_rows / 16;
     const int slice_rows = slices <= 64 ? 4 : (slices <= 1024 ? 16 : 64), ways = slices <= 64 ? 4 : 1;
-    const dim3 grid((unsigned)(blocks * ((p.block_rows + slice_rows - 1) / slice_rows)), (unsigned)p.a.num_kv_heads,
-                    (unsigned)p.num_seqs);
+    const unsigned of_block = (unsigned)((p.block_rows + slice_rows - 1) / slice_rows);
+    const dim3 grid = by_share ? dim3((unsigned)p.groups * of_block)
+                               : dim3((unsigned)blocks * of_block, (unsigned)p.a.num_kv_heads, (unsigned)p.num_seqs);
     if (dtype == kF32)
-        hipLaunchKernelGGL(tree_reduce_kernel<float>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways);
+        hipLaunchKernelGGL(tree_reduce_kernel<float>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways, by_share);
     else
-        hipLaunchKernelGGL(tree_reduce_kernel<f16>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways);
+        hipLaunchKernelGGL(tree_reduce_kernel<f16>, grid, dim3(kTreeReduceThreads), 0, stream, p, slice_rows, ways, by_share);
     return hipGetLastError();
 }
 

@@ -210,19 +210,9 @@ __device__ __forceinline__ void tree_share(const TreeParams &p, const TreeCount 
         }
     }
 }
-// This workgroup's share, and the item that holds its first unit (false: it has none)
-__device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, TreeItem &it) {
+// The item that holds unit u; `n`, `q`: the lane's own of the first 64 sequences
+__device__ __forceinline__ void tree_find(const TreeParams &p, const TreeWork &w, int u, TreeCount n, TreeSeq q, TreeItem &it) {
     const int lane = threadIdx.x & 63;
-    TreeSeq q{};
-    TreeCount n = tree_count(p, lane, q);
-    tree_share(p, n, w);
-    // consecutive shares on one XCD, as row blocks of a kv head read the same keys, and as many
-    // shares on each
-    const int shares = (int)((uint32_t)(w.units + w.per - 1) / (uint32_t)w.per), of_xcd = (shares + kXcds - 1) / kXcds;
-    const int place = blockIdx.x / kXcds;
-    w.group = (int)(blockIdx.x % kXcds) * of_xcd + place;
-    const int u = w.group * w.per;
-    if (place >= of_xcd || u >= w.units) return false;
     int base = 0, s0 = 0;
     for (;;) {
         const int mine = n.items * tree_padded(n.tiles, w.pad);
@@ -249,6 +239,20 @@ __device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, Tre
     it.kvh = (int)((uint32_t)k / (uint32_t)it.blocks);
     it.rb = k - it.kvh * it.blocks;
     it.first = base + k * padded;
+}
+// This workgroup's share, and the item that holds its first unit (false: it has none)
+__device__ __forceinline__ bool tree_start(const TreeParams &p, TreeWork &w, TreeItem &it) {
+    TreeSeq q{};
+    const TreeCount n = tree_count(p, threadIdx.x & 63, q);
+    tree_share(p, n, w);
+    // consecutive shares on one XCD, as row blocks of a kv head read the same keys, and as many
+    // shares on each
+    const int shares = (int)((uint32_t)(w.units + w.per - 1) / (uint32_t)w.per), of_xcd = (shares + kXcds - 1) / kXcds;
+    const int place = blockIdx.x / kXcds;
+    w.group = (int)(blockIdx.x % kXcds) * of_xcd + place;
+    const int u = w.group * w.per;
+    if (place >= of_xcd || u >= w.units) return false;
+    tree_find(p, w, u, n, q, it);
     return true;
 }
 // the end of the share's units of an item, and whether others follow in the share

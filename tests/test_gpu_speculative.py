@@ -549,6 +549,18 @@ def test_tree_attention_forms(dtype, ctx, new, H, K, d, bs, window, words, masks
     b.check(b.run(_engine()))
 
 
+@pytest.mark.parametrize("dtype,H,K,d", [(1, 32, 16, 64), (2, 48, 16, 64), (0, 16, 16, 32)])
+def test_tree_attention_of_more_items_than_workgroups(dtype, H, K, d):
+    """66 sequences, some without rows, of uneven lengths: shares that begin and end inside items, two boundaries in one
+    item, and items that no boundary cuts."""
+    rng = np.random.default_rng(H + d)
+    ctx = [int(x) for x in rng.integers(0, 60, 66)]
+    new = [int(x) for x in rng.integers(0, 12, 66)]
+    ctx[7], new[7], ctx[60], new[60] = 4000, 9, 2500, 11
+    b = Batch(rng, dtype, ctx, new, H, K, d, 16, 0, 1, "tree", spare=1)
+    b.check(b.run(_engine()))
+
+
 @pytest.mark.parametrize("ctx,new,d,bs", [([700, 9], [64, 40], 64, 8), ([700, 9], [64, 40], 128, 4),
                                           ([90], [20], 48, 4), ([90], [20], 64, 2), ([200], [4], 64, 8)])
 def test_tree_attention_of_small_e4m3_blocks(ctx, new, d, bs):
